@@ -244,6 +244,133 @@ TJ_API int tj_flash_attn_fwd_partial(const void* q16, const void* k16, const voi
                               int64_t ld_ctx, float* part_o, float* part_lse, int part_mode,
                               void* stream);
 
+/* ---- expert feed-forward (no reference counterpart) ----------------------
+ *
+ * A feed-forward layer of E experts: each token's top_k experts run the
+ * layer's FFN (ffn_in, erf-GELU, ffn_out) on it and the token's output is
+ * their weighted sum.  tj_route_experts chooses and sorts, tj_gemm_experts
+ * multiplies, tj_expert_combine sums; tj_expert_ffn runs the last two.
+ * Layouts: logits [rows, E]; experts int32 and weights float32 [rows, top_k];
+ * activations and weights float16 or bfloat16, weights [E, N, K] (nn.Linear
+ * layout per expert), biases float32 [E, N].  "Slots" are the (row, j) pairs
+ * sorted by expert, in (row, j) order inside an expert.
+ */
+#define TJ_DTYPE_F32 0
+#define TJ_DTYPE_F16 1
+#define TJ_DTYPE_BF16 2
+
+#define TJ_SCORE_SOFTMAX 0
+#define TJ_SCORE_SIGMOID 1
+
+/* Number of int32 entries of the plan for `rows` rows of top_k choices (0 on
+ * bad arguments); its layout:
+ *   plan[0 .. E]                       offsets: expert e has the slots
+ *                                      [offsets[e], offsets[e+1])
+ *   plan[E+1 .. E+1+rows*top_k)        slot -> row, -1 past the last slot
+ *   plan[E+1+rows*top_k .. +rows*top_k) (row, j) -> slot, -1 without an expert
+ *   the rest                           scratch */
+TJ_API int64_t tj_expert_plan_ints(int rows, int top_k, int num_experts);
+
+/* Routes each row to its top_k of num_experts (at most 512, top_k at most 32).
+ * Scores s: softmax of the row's logits (TJ_SCORE_SOFTMAX) or 1/(1+exp(-x))
+ * (TJ_SCORE_SIGMOID).  Values v = s + bias (bias [E], may be NULL).  With
+ * num_groups > 1 the experts are cut into equal groups (at most 32), a
+ * group's strength is the sum of its group_score_top (1 or 2) greatest
+ * values, and only experts of the top_groups strongest groups stay.  The
+ * top_k greatest values are chosen, greatest first; equal values (and groups)
+ * in index order, and the order of values is that of real arithmetic, not of
+ * their fp32 roundings.  weights = s of the chosen (without bias), divided by
+ * their sum if renormalize, times weight_scale.
+ * A logit of -inf closes an expert to the row: it has no part in the softmax
+ * and is never chosen.  A row with fewer than top_k open experts has experts
+ * -1 and weights 0 in its last places.  A row with a NaN logit (or +inf under
+ * softmax) has NaN weights; its experts are valid indices or -1.
+ * Rows at or past *row_count (NULL = rows) get experts -1 and weights 0.
+ * experts, weights and plan are outputs, all entries written. */
+TJ_API int tj_route_experts(const void* logits, int dtype, int rows, const int32_t* row_count,
+                     int num_experts, int top_k, int scoring, const float* bias, int num_groups,
+                     int top_groups, int group_score_top, int renormalize, float weight_scale,
+                     int32_t* experts, float* weights, int32_t* plan, void* stream);
+
+/* The plan of choices made elsewhere: experts [rows, top_k], negative = none;
+ * an index >= num_experts is recorded as a device error and counts as none.
+ * A row may name an expert twice. */
+TJ_API int tj_expert_plan(const int32_t* experts, int rows, int top_k, const int32_t* row_count,
+                   int num_experts, int32_t* plan, void* stream);
+
+/* out[s] = act(w[e] a[r] + bias[e]) for every slot s of the plan, e its expert
+ * and r = its row (gathered != 0: a is [rows, k]) or s (a is [rows*top_k, k]);
+ * act is erf-GELU on the fp32 sum if gelu != 0, else nothing.  out is
+ * [rows*top_k, n]; entries past the plan's last slot stay as they were.  n and
+ * k multiples of 8, pointers 16-byte aligned, bias may be NULL. */
+TJ_API int tj_gemm_experts(const void* a, int dtype, int gathered, const void* w, const float* bias,
+                    const int32_t* plan, int rows, int top_k, int num_experts, int n, int k, int gelu,
+                    void* out, void* stream);
+
+/* out[r] = sum over j of weights[r, j] * y[slot(r, j)], summed in fp32 and
+ * rounded once; zeros for a row without experts.  Rows at or past *row_count
+ * stay as they were.  d_model a multiple of 8. */
+TJ_API int tj_expert_combine(const void* y, int dtype, const float* weights, const int32_t* plan,
+                      const int32_t* row_count, int rows, int top_k, int num_experts, int d_model,
+                      void* out, void* stream);
+
+/* Workspace bytes tj_expert_ffn needs (0 on bad arguments). */
+TJ_API int64_t tj_expert_ffn_workspace_bytes(int rows, int top_k, int d_model, int ffn_dim);
+
+/* out [rows, d_model] = the routed feed-forward of a [rows, d_model]:
+ * w_in [E, ffn_dim, d_model], w_out [E, d_model, ffn_dim]; the hidden layer
+ * and each expert's output are rounded to `dtype` once, as the dense FFN's. */
+TJ_API int tj_expert_ffn(const void* a, int dtype, const void* w_in, const float* b_in, const void* w_out,
+                  const float* b_out, const float* weights, const int32_t* plan,
+                  const int32_t* row_count, int rows, int top_k, int num_experts, int d_model,
+                  int ffn_dim, void* out, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- residual step with a norm behind the block and one before the next --- */
+
+#define TJ_GATE_NONE 0
+#define TJ_GATE_SIGMOID 1
+#define TJ_GATE_TANH 2
+
+/* For r < min(rows, *row_count):
+ *   b = branch16[r], or with weights (an expert layer's outputs in slot order)
+ *       sum over j of weights[r, j] * branch16[row_slot[r, j]], skipping
+ *       negative slots
+ *   p = post norm of b (post_gamma NULL: p = b)
+ *   s = x[row_map ? row_map[r] : r] + residual_scale * act(gate) * p
+ *   sum_out[r] = s (if sum_out is not NULL);  y16[r] = pre norm of s
+ * Norms are LayerNorm, or RMSNorm with rms != 0 (beta NULL = 0), eps inside
+ * the root; all arithmetic in fp32, y16 rounded to `dtype` once.  The gate row
+ * is (gate_map ? gate_map[r] : r) / rows_per_gate: gate [1, D] with
+ * rows_per_gate >= rows for a gate per channel, rows_per_gate = seq_len for
+ * one per sample, 1 for one per row.  d_model up to 32768 (8192 when it is not
+ * a multiple of 8 or a pointer is not 16-byte aligned).  sum_out may be x
+ * itself when row_map is NULL.  A row map entry or gate row outside its buffer
+ * is recorded as a device error and the row is left out. */
+typedef struct tj_sandwich_desc {
+  const float* x;           /* [x_rows, D] */
+  const int32_t* row_map;   /* [rows] or NULL */
+  const void* branch16;     /* [branch_rows, D] */
+  const float* weights;     /* [rows, top_k] or NULL */
+  const int32_t* row_slot;  /* [rows, top_k], with weights */
+  const float* post_gamma;  /* [D] or NULL: no norm of the branch */
+  const float* post_beta;   /* [D] or NULL */
+  const void* gate;         /* [gate_rows, D] or NULL: 1 */
+  const int32_t* gate_map;  /* [rows] or NULL */
+  const float* pre_gamma;   /* [D] */
+  const float* pre_beta;    /* [D] or NULL */
+  const int32_t* row_count; /* device int or NULL */
+  float* sum_out;           /* [rows, D] or NULL */
+  void* y16;                /* [rows, D] */
+  int64_t branch_rows;
+  int dtype;                /* of branch16 and y16: TJ_DTYPE_F16 or TJ_DTYPE_BF16 */
+  int rows, x_rows, d_model, top_k;
+  int gate_rows, rows_per_gate, gate_dtype, gate_act;
+  int rms;
+  float eps, residual_scale;
+} tj_sandwich_desc;
+
+TJ_API int tj_sandwich_norm(const tj_sandwich_desc* desc, void* stream);
+
 /* ---- whole encoder ----------------------------------------------------- */
 
 typedef struct tj_encoder_desc {

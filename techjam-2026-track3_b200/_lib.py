@@ -80,6 +80,50 @@ class LayerWeights(ctypes.Structure):
     ]
 
 
+TJ_DTYPE_F32 = 0
+TJ_DTYPE_F16 = 1
+TJ_DTYPE_BF16 = 2
+
+TJ_SCORE_SOFTMAX = 0
+TJ_SCORE_SIGMOID = 1
+
+TJ_GATE_NONE = 0
+TJ_GATE_SIGMOID = 1
+TJ_GATE_TANH = 2
+
+
+class SandwichDesc(ctypes.Structure):
+    _fields_ = [
+        ("x", c_vp),
+        ("row_map", c_vp),
+        ("branch16", c_vp),
+        ("weights", c_vp),
+        ("row_slot", c_vp),
+        ("post_gamma", c_vp),
+        ("post_beta", c_vp),
+        ("gate", c_vp),
+        ("gate_map", c_vp),
+        ("pre_gamma", c_vp),
+        ("pre_beta", c_vp),
+        ("row_count", c_vp),
+        ("sum_out", c_vp),
+        ("y16", c_vp),
+        ("branch_rows", c_i64),
+        ("dtype", c_int),
+        ("rows", c_int),
+        ("x_rows", c_int),
+        ("d_model", c_int),
+        ("top_k", c_int),
+        ("gate_rows", c_int),
+        ("rows_per_gate", c_int),
+        ("gate_dtype", c_int),
+        ("gate_act", c_int),
+        ("rms", c_int),
+        ("eps", c_float),
+        ("residual_scale", c_float),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/techjam_b200.h declares.
 SIGNATURES = {
     "tj_abi_version": (c_int, []),
@@ -134,6 +178,29 @@ SIGNATURES = {
             c_vp, c_vp, c_vp, c_float, c_int, c_vp, c_vp, c_i64, c_vp, c_vp, c_int, c_vp,
         ],
     ),
+    "tj_expert_plan_ints": (c_i64, [c_int, c_int, c_int]),
+    "tj_route_experts": (
+        c_int,
+        [
+            c_vp, c_int, c_int, c_vp, c_int, c_int, c_int, c_vp, c_int, c_int, c_int, c_int, c_float,
+            c_vp, c_vp, c_vp, c_vp,
+        ],
+    ),
+    "tj_expert_plan": (c_int, [c_vp, c_int, c_int, c_vp, c_int, c_vp, c_vp]),
+    "tj_gemm_experts": (
+        c_int,
+        [c_vp, c_int, c_int, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int, c_int, c_vp, c_vp],
+    ),
+    "tj_expert_combine": (c_int, [c_vp, c_int, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_vp, c_vp]),
+    "tj_expert_ffn_workspace_bytes": (c_i64, [c_int, c_int, c_int, c_int]),
+    "tj_expert_ffn": (
+        c_int,
+        [
+            c_vp, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int,
+            c_vp, c_vp, c_i64, c_vp,
+        ],
+    ),
+    "tj_sandwich_norm": (c_int, [ctypes.POINTER(SandwichDesc), c_vp]),
     "tj_encoder_workspace_bytes": (c_i64, [ctypes.POINTER(EncoderDesc)]),
     "tj_encoder_forward": (
         c_int,

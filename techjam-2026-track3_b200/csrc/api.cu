@@ -16,6 +16,9 @@
 #include "gemm_tcgen05.cu"
 #include "attention_tcgen05.cu"
 #include "small_encoder.cu"
+#include "experts_route.cu"
+#include "sandwich_norm.cu"
+#include "experts_gemm.cu"
 
 namespace tj {
 
@@ -370,6 +373,178 @@ int tj_flash_attn_fwd(const void* q16, const void* k16, const void* v16, int num
   return tj_flash_attn_fwd_strided(q16, k16, v16, num_heads, head_dim, q_rows, kv_rows, kv_stride_h,
                                    kv_stride_g, num_segments, batch, max_q_per_sample, q_cu, kv_off,
                                    kv_len, scale, causal, q_pos0, ctx16, 0, stream);
+}
+
+int64_t tj_expert_plan_ints(int rows, int top_k, int num_experts) {
+  if (rows < 0 || top_k < 1 || num_experts < 1) return 0;
+  return expert_plan_ints(rows, top_k, num_experts);
+}
+
+int tj_route_experts(const void* logits, int dtype, int rows, const int32_t* row_count,
+                     int num_experts, int top_k, int scoring, const float* bias, int num_groups,
+                     int top_groups, int group_score_top, int renormalize, float weight_scale,
+                     int32_t* experts, float* weights, int32_t* plan, void* stream) {
+  int rc = check_device();
+  if (rc) return rc;
+  RouteArgs a{};
+  // without rows there may be no logits; the plan is then all empty
+  if (!logits && rows != 0) return set_error(TJ_ERR_INVALID_ARGUMENT, "route_experts: null logits");
+  a.logits = logits;
+  a.dtype = dtype;
+  a.rows = rows;
+  a.row_count = row_count;
+  a.num_experts = num_experts;
+  a.top_k = top_k;
+  a.scoring = scoring;
+  a.bias = bias;
+  a.groups = num_groups;
+  a.top_groups = top_groups;
+  a.group_top = group_score_top;
+  a.renormalize = renormalize;
+  a.weight_scale = weight_scale;
+  a.experts = experts;
+  a.weights = weights;
+  a.plan = plan;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return finish(launch_route(a, s), s);
+}
+
+int tj_expert_plan(const int32_t* experts, int rows, int top_k, const int32_t* row_count,
+                   int num_experts, int32_t* plan, void* stream) {
+  int rc = check_device();
+  if (rc) return rc;
+  RouteArgs a{};
+  a.rows = rows;
+  a.row_count = row_count;
+  a.num_experts = num_experts;
+  a.top_k = top_k;
+  a.groups = a.top_groups = a.group_top = 1;
+  a.experts = const_cast<int32_t*>(experts);  // only read without logits
+  a.plan = plan;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return finish(launch_route(a, s), s);
+}
+
+// Views of a plan buffer.
+static const int32_t* plan_slot_row(const int32_t* plan, int num_experts) { return plan + num_experts + 1; }
+static const int32_t* plan_row_slot(const int32_t* plan, int num_experts, int rows, int top_k) {
+  return plan + num_experts + 1 + (int64_t)rows * top_k;
+}
+
+static int check_expert_shape(const char* what, int rows, int top_k, int num_experts) {
+  if (rows < 0 || top_k < 1 || top_k > kRouteMaxTopK || num_experts < 1 || num_experts > kRouteMaxExperts ||
+      2 * (int64_t)rows * top_k > INT32_MAX)
+    return set_error(TJ_ERR_INVALID_ARGUMENT, "%s: rows=%d top_k=%d num_experts=%d", what, rows, top_k, num_experts);
+  return TJ_OK;
+}
+
+int tj_gemm_experts(const void* a, int dtype, int gathered, const void* w, const float* bias,
+                    const int32_t* plan, int rows, int top_k, int num_experts, int n, int k, int gelu,
+                    void* out, void* stream) {
+  int rc = check_device();
+  if (rc) return rc;
+  rc = check_expert_shape("gemm_experts", rows, top_k, num_experts);
+  if (rc) return rc;
+  if (!plan) return set_error(TJ_ERR_INVALID_ARGUMENT, "gemm_experts: null plan");
+  ExpertGemmArgs g{};
+  g.a = a;
+  g.w = w;
+  g.bias = bias;
+  g.offsets = plan;
+  g.slot_row = plan_slot_row(plan, num_experts);
+  g.dtype = dtype;
+  g.gather = gathered != 0;
+  g.gelu = gelu != 0;
+  g.slots = rows * top_k;
+  g.a_rows = gathered ? rows : g.slots;
+  g.num_experts = num_experts;
+  g.N = n;
+  g.K = k;
+  g.out = out;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return finish(launch_experts_gemm(g, s), s);
+}
+
+int tj_expert_combine(const void* y, int dtype, const float* weights, const int32_t* plan,
+                      const int32_t* row_count, int rows, int top_k, int num_experts, int d_model,
+                      void* out, void* stream) {
+  int rc = check_device();
+  if (rc) return rc;
+  rc = check_expert_shape("expert_combine", rows, top_k, num_experts);
+  if (rc) return rc;
+  if (!plan) return set_error(TJ_ERR_INVALID_ARGUMENT, "expert_combine: null plan");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return finish(launch_expert_combine(dtype, y, weights, plan_row_slot(plan, num_experts, rows, top_k), row_count,
+                                      rows, top_k, d_model, out, s),
+                s);
+}
+
+int64_t tj_expert_ffn_workspace_bytes(int rows, int top_k, int d_model, int ffn_dim) {
+  if (rows < 0 || top_k < 1 || d_model <= 0 || ffn_dim <= 0) return 0;
+  const size_t slots = (size_t)rows * top_k;
+  return (int64_t)(align_up(slots * ffn_dim * 2, 256) + align_up(slots * d_model * 2, 256));
+}
+
+int tj_expert_ffn(const void* a, int dtype, const void* w_in, const float* b_in, const void* w_out,
+                  const float* b_out, const float* weights, const int32_t* plan,
+                  const int32_t* row_count, int rows, int top_k, int num_experts, int d_model,
+                  int ffn_dim, void* out, void* workspace, int64_t workspace_bytes, void* stream) {
+  int rc = check_device();
+  if (rc) return rc;
+  rc = check_expert_shape("expert_ffn", rows, top_k, num_experts);
+  if (rc) return rc;
+  if (d_model <= 0 || ffn_dim <= 0 || d_model % 8 != 0 || ffn_dim % 8 != 0)
+    return set_error(TJ_ERR_UNSUPPORTED, "expert_ffn: d_model=%d and ffn_dim=%d must be multiples of 8", d_model, ffn_dim);
+  if (!plan) return set_error(TJ_ERR_INVALID_ARGUMENT, "expert_ffn: null plan");
+  if (rows == 0) return TJ_OK;
+  const int64_t need = tj_expert_ffn_workspace_bytes(rows, top_k, d_model, ffn_dim);
+  if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u))
+    return set_error(TJ_ERR_WORKSPACE, "expert_ffn: workspace of %lld bytes (256-byte aligned), %lld needed",
+                     (long long)workspace_bytes, (long long)need);
+  const int slots = rows * top_k;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  void* h16 = ws;
+  void* y16 = ws + align_up((size_t)slots * ffn_dim * 2, 256);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  ExpertGemmArgs g{};
+  g.a = a;
+  g.w = w_in;
+  g.bias = b_in;
+  g.offsets = plan;
+  g.slot_row = plan_slot_row(plan, num_experts);
+  g.dtype = dtype;
+  g.gather = 1;
+  g.gelu = 1;
+  g.slots = slots;
+  g.a_rows = rows;
+  g.num_experts = num_experts;
+  g.N = ffn_dim;
+  g.K = d_model;
+  g.out = h16;
+  rc = launch_experts_gemm(g, s);
+  if (rc) return rc;
+  g.a = h16;
+  g.w = w_out;
+  g.bias = b_out;
+  g.gather = 0;
+  g.gelu = 0;
+  g.a_rows = slots;
+  g.N = d_model;
+  g.K = ffn_dim;
+  g.out = y16;
+  rc = launch_experts_gemm(g, s);
+  if (rc) return rc;
+  return finish(launch_expert_combine(dtype, y16, weights, plan_row_slot(plan, num_experts, rows, top_k), row_count,
+                                      rows, top_k, d_model, out, s),
+                s);
+}
+
+int tj_sandwich_norm(const tj_sandwich_desc* desc, void* stream) {
+  int rc = check_device();
+  if (rc) return rc;
+  if (!desc) return set_error(TJ_ERR_INVALID_ARGUMENT, "sandwich_norm: null descriptor");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return finish(launch_sandwich_norm(*desc, s), s);
 }
 
 int64_t tj_encoder_workspace_bytes(const tj_encoder_desc* desc) {

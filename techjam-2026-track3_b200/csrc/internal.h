@@ -138,4 +138,39 @@ int launch_attention(const AttnArgs& args, cudaStream_t stream);
 // 128 or 256 (heads are zero-padded up to it).
 int attn_head_pad(int head_dim);
 
+// Router and plan of the expert feed-forward (experts_route.cu).  logits null:
+// the plan of the given choices.
+struct RouteArgs {
+  const void* logits;
+  int dtype, rows;
+  const int32_t* row_count;
+  int num_experts, top_k, scoring;
+  const float* bias;
+  int groups, top_groups, group_top, renormalize;
+  float weight_scale;
+  int32_t* experts;
+  float* weights;
+  int32_t* plan;
+};
+int64_t expert_plan_ints(int rows, int top_k, int num_experts);
+int launch_route(const RouteArgs& args, cudaStream_t stream);
+
+// out[s] = act(W[e] a[gather ? slot_row[s] : s] + bias[e]) over a plan's slots.
+struct ExpertGemmArgs {
+  const void* a;            // [a_rows][K]
+  const void* w;            // [num_experts][N][K]
+  const float* bias;        // [num_experts][N] or null
+  const int32_t* offsets;   // [num_experts+1]
+  const int32_t* slot_row;  // [slots]
+  int dtype, gather, gelu;
+  int slots, a_rows, num_experts, N, K;
+  void* out;                // [slots][N]
+};
+int launch_experts_gemm(const ExpertGemmArgs& args, cudaStream_t stream);
+
+int launch_expert_combine(int dtype, const void* y, const float* weights, const int32_t* row_slot,
+                          const int32_t* row_count, int rows, int top_k, int D, void* out, cudaStream_t stream);
+
+int launch_sandwich_norm(const tj_sandwich_desc& desc, cudaStream_t stream);
+
 }  // namespace tj

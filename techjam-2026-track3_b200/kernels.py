@@ -10,6 +10,7 @@ tj_encoder_forward entry point.
 from __future__ import annotations
 
 import ctypes
+from dataclasses import dataclass
 from typing import Optional
 
 import torch
@@ -348,3 +349,354 @@ def flash_attn_fwd(q, k, v, q_cu, kv_off, kv_len, max_q_per_sample, scale, causa
     )
     _lib.check(rc, "flash_attn_fwd")
     return out
+
+
+# ---- expert feed-forward ------------------------------------------------------
+_DTYPES = {torch.float32: _lib.TJ_DTYPE_F32, torch.float16: _lib.TJ_DTYPE_F16, torch.bfloat16: _lib.TJ_DTYPE_BF16}
+_SCORES = {"softmax": _lib.TJ_SCORE_SOFTMAX, "sigmoid": _lib.TJ_SCORE_SIGMOID}
+_GATES = {"none": _lib.TJ_GATE_NONE, "sigmoid": _lib.TJ_GATE_SIGMOID, "tanh": _lib.TJ_GATE_TANH}
+
+
+def _no_grad(*tensors) -> None:
+    """Forward only, like the encoder: a call whose gradient would be lost raises."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("autograd through this operator is not supported; call it under torch.no_grad()")
+
+
+def _cuda_tensor(t, name: str) -> torch.device:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if t.device.type != "cuda":
+        raise ValueError(f"{name} must be a CUDA tensor (the library has no CPU path)")
+    return t.device
+
+
+def _require_shape(t, name: str, shape, dtype: torch.dtype, device: torch.device) -> None:
+    _require(t, name, dtype, device)
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _require_count(row_count, device: torch.device) -> None:
+    if row_count is not None:
+        _require(row_count, "row_count", torch.int32, device)
+        if row_count.numel() != 1:
+            raise ValueError("row_count must hold one int32")
+
+
+def _half_dtype(t: torch.Tensor, name: str) -> int:
+    if t.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"{name} must be float16 or bfloat16, got {t.dtype}")
+    return _DTYPES[t.dtype]
+
+
+@dataclass
+class ExpertRouting:
+    """Choices of a batch of rows and the plan the expert kernels read: `experts`
+    [rows, top_k] int32 (-1: none), `weights` [rows, top_k] float32, and
+    `plan`, whose parts are the properties below.  Slots are the (row, j)
+    pairs sorted by expert, in (row, j) order inside an expert.  `row_count`
+    is the device int given to the router (None: all rows)."""
+
+    experts: torch.Tensor
+    weights: torch.Tensor
+    plan: torch.Tensor
+    num_experts: int
+    row_count: Optional[torch.Tensor] = None
+
+    @property
+    def rows(self) -> int:
+        return self.experts.shape[0]
+
+    @property
+    def top_k(self) -> int:
+        return self.experts.shape[1]
+
+    @property
+    def offsets(self) -> torch.Tensor:
+        """[num_experts + 1]: expert e has slots offsets[e] .. offsets[e+1]."""
+        return self.plan[: self.num_experts + 1]
+
+    @property
+    def slot_row(self) -> torch.Tensor:
+        """[rows * top_k]: row of each slot, -1 past the last slot."""
+        n = self.num_experts + 1
+        return self.plan[n : n + self.rows * self.top_k]
+
+    @property
+    def row_slot(self) -> torch.Tensor:
+        """[rows, top_k]: slot of each choice, -1 without an expert."""
+        n, s = self.num_experts + 1, self.rows * self.top_k
+        return self.plan[n + s : n + 2 * s].view(self.rows, self.top_k)
+
+
+def _plan_buffer(rows: int, top_k: int, num_experts: int, device: torch.device) -> torch.Tensor:
+    n = _lib.load().tj_expert_plan_ints(rows, top_k, num_experts)
+    return torch.empty(n, dtype=torch.int32, device=device)
+
+
+def route_experts(logits, top_k, *, scoring="softmax", bias=None, num_groups=1, top_groups=1, group_score_top=1,
+                  renormalize=True, weight_scale=1.0, row_count=None) -> ExpertRouting:
+    """Routes each row of logits [rows, E] (float32, float16 or bfloat16) to its
+    top_k experts and sorts the choices by expert.
+
+    Scores are the row's softmax or sigmoid; the experts with the greatest
+    score + bias (bias: [E] float32) are chosen, equal values in index order,
+    and with num_groups > 1 only among the top_groups groups with the greatest
+    sum of their group_score_top (1 or 2) best values.  Weights are the scores
+    of the chosen, divided by their sum if renormalize, times weight_scale.  A
+    logit of -inf closes an expert to the row (a row without enough open
+    experts ends in -1 with weight 0), a row with a NaN has NaN weights, and
+    rows at or past row_count (a device int32) are not routed."""
+    dev = _cuda_tensor(logits, "logits")
+    _no_grad(logits, bias)
+    if logits.dtype not in _DTYPES:
+        raise TypeError(f"logits must be float32, float16 or bfloat16, got {logits.dtype}")
+    _require(logits, "logits", logits.dtype, dev)
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be [rows, experts], got {tuple(logits.shape)}")
+    rows, E = logits.shape
+    if scoring not in _SCORES:
+        raise ValueError(f"scoring must be one of {sorted(_SCORES)}, got {scoring!r}")
+    if not 1 <= top_k <= min(E, 32):
+        raise ValueError(f"top_k must be in 1..{min(E, 32)}, got {top_k}")
+    if bias is not None:
+        _require_shape(bias, "bias", (E,), torch.float32, dev)
+    _require_count(row_count, dev)
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        experts = torch.empty(rows, top_k, dtype=torch.int32, device=dev)
+        weights = torch.empty(rows, top_k, dtype=torch.float32, device=dev)
+        plan = _plan_buffer(rows, top_k, E, dev)
+        rc = lib.tj_route_experts(
+            logits.data_ptr(), _DTYPES[logits.dtype], rows, _ptr(row_count), E, top_k, _SCORES[scoring], _ptr(bias),
+            num_groups, top_groups, group_score_top, 1 if renormalize else 0, float(weight_scale), experts.data_ptr(),
+            weights.data_ptr(), plan.data_ptr(), _stream(logits),
+        )
+    _lib.check(rc, "route_experts")
+    return ExpertRouting(experts, weights, plan, E, row_count)
+
+
+def expert_plan(experts, weights, num_experts, *, row_count=None) -> ExpertRouting:
+    """Routing made of choices from elsewhere: experts [rows, top_k] int32
+    (negative: none; a row may name an expert twice) and weights [rows, top_k]
+    float32.  An index >= num_experts is a device error and counts as none."""
+    dev = _cuda_tensor(experts, "experts")
+    _no_grad(weights)
+    _require(experts, "experts", torch.int32, dev)
+    if experts.dim() != 2 or not 1 <= experts.shape[1] <= 32:
+        raise ValueError(f"experts must be [rows, top_k] with top_k in 1..32, got {tuple(experts.shape)}")
+    rows, top_k = experts.shape
+    _require_shape(weights, "weights", (rows, top_k), torch.float32, dev)
+    _require_count(row_count, dev)
+    if not 1 <= num_experts <= 512:
+        raise ValueError(f"num_experts must be in 1..512, got {num_experts}")
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        plan = _plan_buffer(rows, top_k, num_experts, dev)
+        rc = lib.tj_expert_plan(experts.data_ptr(), rows, top_k, _ptr(row_count), num_experts, plan.data_ptr(),
+                                _stream(experts))
+    _lib.check(rc, "expert_plan")
+    return ExpertRouting(experts, weights, plan, num_experts, row_count)
+
+
+def _require_routing(routing, device: torch.device) -> None:
+    if not isinstance(routing, ExpertRouting):
+        raise TypeError("routing must be an ExpertRouting (route_experts, expert_plan)")
+    if routing.plan.device != device:
+        raise ValueError(f"routing must be on {device}, got {routing.plan.device}")
+
+
+def gemm_experts(a, w, bias, routing, *, gather, gelu=False, out=None):
+    """out[s] = act(w[e] @ a[r] + bias[e]) for every slot s of the routing, e its
+    expert and r its row (gather: a is [rows, K]) or s (a is [rows * top_k, K]);
+    act is erf-GELU or none.  w [E, N, K], bias [E, N] float32 or None, N and K
+    multiples of 8.  Rows of out [rows * top_k, N] past the last slot are left
+    as they were."""
+    dev = _cuda_tensor(a, "a")
+    _no_grad(a, w, bias)
+    code = _half_dtype(a, "a")
+    _require_routing(routing, dev)
+    slots = routing.rows * routing.top_k
+    if a.dim() != 2:
+        raise ValueError(f"a must be a matrix, got {tuple(a.shape)}")
+    K = a.shape[1]
+    _require_shape(a, "a", (routing.rows if gather else slots, K), a.dtype, dev)
+    _require(w, "w", a.dtype, dev)
+    if w.dim() != 3 or w.shape[0] != routing.num_experts or w.shape[2] != K:
+        raise ValueError(f"w must be [{routing.num_experts}, N, {K}], got {tuple(w.shape)}")
+    N = w.shape[1]
+    if bias is not None:
+        _require_shape(bias, "bias", (routing.num_experts, N), torch.float32, dev)
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        if out is None:
+            out = torch.empty(slots, N, dtype=a.dtype, device=dev)
+        _require_out(out, "out", (slots, N), a.dtype, dev)
+        rc = lib.tj_gemm_experts(
+            a.data_ptr(), code, 1 if gather else 0, w.data_ptr(), _ptr(bias), routing.plan.data_ptr(), routing.rows,
+            routing.top_k, routing.num_experts, N, K, 1 if gelu else 0, out.data_ptr(), _stream(a),
+        )
+    _lib.check(rc, "gemm_experts")
+    return out
+
+
+def expert_combine(y, routing, *, out=None):
+    """out[r] = sum_j weights[r, j] * y[slot(r, j)], zeros for a row without
+    experts; rows at or past the routing's row_count are left as they were."""
+    dev = _cuda_tensor(y, "y")
+    _no_grad(y, routing.weights if isinstance(routing, ExpertRouting) else None)
+    code = _half_dtype(y, "y")
+    _require_routing(routing, dev)
+    if y.dim() != 2:
+        raise ValueError(f"y must be a matrix, got {tuple(y.shape)}")
+    D = y.shape[1]
+    _require_shape(y, "y", (routing.rows * routing.top_k, D), y.dtype, dev)
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        if out is None:
+            out = torch.empty(routing.rows, D, dtype=y.dtype, device=dev)
+        _require_out(out, "out", (routing.rows, D), y.dtype, dev)
+        rc = lib.tj_expert_combine(
+            y.data_ptr(), code, routing.weights.data_ptr(), routing.plan.data_ptr(), _ptr(routing.row_count),
+            routing.rows, routing.top_k, routing.num_experts, D, out.data_ptr(), _stream(y),
+        )
+    _lib.check(rc, "expert_combine")
+    return out
+
+
+def expert_ffn(a, w_in, b_in, w_out, b_out, routing, *, out=None):
+    """The routed feed-forward of a [rows, D] (float16 or bfloat16): each row's
+    experts run ffn_in, erf-GELU and ffn_out on it and out is their weighted
+    sum.  w_in [E, F, D], w_out [E, D, F], biases [E, F] and [E, D] float32 or
+    None, D and F multiples of 8.  Zeros for a row without experts; rows at or
+    past the routing's row_count are left as they were."""
+    dev = _cuda_tensor(a, "a")
+    _no_grad(a, w_in, b_in, w_out, b_out)
+    code = _half_dtype(a, "a")
+    _require_routing(routing, dev)
+    E = routing.num_experts
+    if a.dim() != 2 or a.shape[0] != routing.rows:
+        raise ValueError(f"a must be [{routing.rows}, D], got {tuple(a.shape)}")
+    _require(a, "a", a.dtype, dev)
+    D = a.shape[1]
+    _require(w_in, "w_in", a.dtype, dev)
+    if w_in.dim() != 3 or w_in.shape[0] != E or w_in.shape[2] != D:
+        raise ValueError(f"w_in must be [{E}, F, {D}], got {tuple(w_in.shape)}")
+    F = w_in.shape[1]
+    _require_shape(w_out, "w_out", (E, D, F), a.dtype, dev)
+    if b_in is not None:
+        _require_shape(b_in, "b_in", (E, F), torch.float32, dev)
+    if b_out is not None:
+        _require_shape(b_out, "b_out", (E, D), torch.float32, dev)
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        if out is None:
+            out = torch.empty(routing.rows, D, dtype=a.dtype, device=dev)
+        _require_out(out, "out", (routing.rows, D), a.dtype, dev)
+        need = lib.tj_expert_ffn_workspace_bytes(routing.rows, routing.top_k, D, F)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        rc = lib.tj_expert_ffn(
+            a.data_ptr(), code, w_in.data_ptr(), _ptr(b_in), w_out.data_ptr(), _ptr(b_out),
+            routing.weights.data_ptr(), routing.plan.data_ptr(), _ptr(routing.row_count), routing.rows, routing.top_k,
+            E, D, F, out.data_ptr(), ws.data_ptr(), need, _stream(a),
+        )
+    _lib.check(rc, "expert_ffn")
+    return out
+
+
+def sandwich_norm(x, branch, pre_gamma, pre_beta=None, *, post_gamma=None, post_beta=None, kind="layer", gate=None,
+                  gate_act="none", rows_per_gate=1, gate_map=None, residual_scale=1.0, eps=1e-5, row_map=None,
+                  row_count=None, routing=None, sum_out=None, out=None):
+    """The residual step between two blocks, with a norm behind one and a norm
+    before the next:
+
+        s[r] = x[row_map[r]] + residual_scale * act(gate) * post(b[r])
+        y[r] = pre(s[r])
+
+    returning (s float32, y in branch's dtype).  b is branch [rows, D] (float16
+    or bfloat16), or with `routing` the weighted sum of branch [rows * top_k,
+    D], its experts' outputs in slot order.  post and pre are LayerNorm
+    (kind="layer") or RMSNorm ("rms"); no post_gamma: no norm of the branch.
+    gate: [D] (float32) per channel, or [G, D] (float32 or branch's dtype) with
+    row r reading gate row gate_map[r] // rows_per_gate (gate_map: int32,
+    default row_map, else r): a sample's gate with rows_per_gate = seq_len, a
+    token's with 1.  act: none, sigmoid or tanh.  x [x_rows, D] float32; sum_out
+    may be x when there is no row_map.  Rows at or past row_count (default:
+    the routing's) are left as they were."""
+    dev = _cuda_tensor(x, "x")
+    _no_grad(x, branch, pre_gamma, pre_beta, post_gamma, post_beta, gate)
+    _require(x, "x", torch.float32, dev)
+    if x.dim() != 2:
+        raise ValueError(f"x must be [rows, D], got {tuple(x.shape)}")
+    D = x.shape[1]
+    _cuda_tensor(branch, "branch")
+    code = _half_dtype(branch, "branch")
+    if kind not in ("layer", "rms"):
+        raise ValueError(f"kind must be 'layer' or 'rms', got {kind!r}")
+    if gate_act not in _GATES:
+        raise ValueError(f"gate_act must be one of {sorted(_GATES)}, got {gate_act!r}")
+    if routing is not None:
+        _require_routing(routing, dev)
+        _no_grad(routing.weights)
+        rows = routing.rows
+        _require_shape(branch, "branch", (rows * routing.top_k, D), branch.dtype, dev)
+        if row_count is None:
+            row_count = routing.row_count
+    else:
+        rows = branch.shape[0]
+        _require_shape(branch, "branch", (rows, D), branch.dtype, dev)
+    _require_count(row_count, dev)
+    if row_map is not None:
+        _require_shape(row_map, "row_map", (rows,), torch.int32, dev)
+    elif x.shape[0] < rows:
+        raise ValueError(f"x must have at least {rows} rows, got {x.shape[0]}")
+    for name, t in (("pre_gamma", pre_gamma), ("pre_beta", pre_beta), ("post_gamma", post_gamma),
+                    ("post_beta", post_beta)):
+        if t is not None:
+            _require_shape(t, name, (D,), torch.float32, dev)
+    if pre_gamma is None:
+        raise ValueError("pre_gamma is required")
+    if post_beta is not None and post_gamma is None:
+        raise ValueError("post_beta needs post_gamma")
+    gate_rows, gate_code = 0, _lib.TJ_DTYPE_F32
+    if gate is not None:
+        if gate.dim() == 1:
+            _require_shape(gate, "gate", (D,), torch.float32, dev)
+            gate_rows, rows_per_gate, gate_map = 1, max(rows, 1), None
+        else:
+            if gate.dtype not in (torch.float32, branch.dtype):
+                raise TypeError(f"gate must be float32 or {branch.dtype}, got {gate.dtype}")
+            _require(gate, "gate", gate.dtype, dev)
+            if gate.dim() != 2 or gate.shape[1] != D or gate.shape[0] < 1:
+                raise ValueError(f"gate must be [{D}] or [G, {D}], got {tuple(gate.shape)}")
+            if rows_per_gate < 1:
+                raise ValueError(f"rows_per_gate must be at least 1, got {rows_per_gate}")
+            gate_rows, gate_code = gate.shape[0], _DTYPES[gate.dtype]
+            if gate_map is None:
+                gate_map = row_map
+            if gate_map is not None:
+                _require_shape(gate_map, "gate_map", (rows,), torch.int32, dev)
+            elif gate_rows * rows_per_gate < rows:
+                raise ValueError(f"gate has {gate_rows} rows of {rows_per_gate} rows each, {rows} rows to gate")
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        if sum_out is None:
+            sum_out = torch.empty(rows, D, dtype=torch.float32, device=dev)
+        _require_out(sum_out, "sum_out", (rows, D), torch.float32, dev)
+        if row_map is not None and sum_out.data_ptr() == x.data_ptr():
+            raise ValueError("sum_out cannot be x when row_map is given")
+        if out is None:
+            out = torch.empty(rows, D, dtype=branch.dtype, device=dev)
+        _require_out(out, "out", (rows, D), branch.dtype, dev)
+        desc = _lib.SandwichDesc(
+            x.data_ptr(), _ptr(row_map), branch.data_ptr(), routing.weights.data_ptr() if routing is not None else None,
+            routing.row_slot.data_ptr() if routing is not None else None, _ptr(post_gamma), _ptr(post_beta),
+            _ptr(gate), _ptr(gate_map), _ptr(pre_gamma), _ptr(pre_beta), _ptr(row_count), sum_out.data_ptr(),
+            out.data_ptr(), branch.shape[0], code, rows, x.shape[0], D, routing.top_k if routing is not None else 0,
+            gate_rows, rows_per_gate, gate_code, _GATES[gate_act], 1 if kind == "rms" else 0, float(eps),
+            float(residual_scale),
+        )
+        rc = lib.tj_sandwich_norm(ctypes.byref(desc), _stream(x))
+    _lib.check(rc, "sandwich_norm")
+    return sum_out, out

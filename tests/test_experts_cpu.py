@@ -1,0 +1,173 @@
+"""Refusals of the expert and sandwich-norm entry points, without a GPU: the
+device check is replaced so CPU tensors pass it, and the library must not be
+reached."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+F16, F32, I32 = torch.float16, torch.float32, torch.int32
+
+
+class _Unreached(Exception):
+    pass
+
+
+@pytest.fixture
+def k(pkg, monkeypatch):
+    kern = pkg.kernels
+
+    def device(t, name):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a tensor")
+        return t.device
+
+    def load():
+        raise _Unreached
+
+    monkeypatch.setattr(kern, "_cuda_tensor", device)
+    monkeypatch.setattr(kern._lib, "load", load)
+    return kern
+
+
+def test_cpu_tensors_are_refused(pkg):
+    kern = pkg.kernels
+    with pytest.raises(ValueError, match="CUDA"):
+        kern.route_experts(torch.zeros(2, 4), 1)
+    with pytest.raises(ValueError, match="CUDA"):
+        kern.sandwich_norm(torch.zeros(2, 8), torch.zeros(2, 8, dtype=F16), torch.ones(8))
+    with pytest.raises(TypeError):
+        kern.route_experts([[1.0]], 1)
+
+
+def test_plan_and_workspace_sizes(pkg):
+    lib = pkg._lib.load()
+    assert lib.tj_expert_plan_ints(0, 2, 8) == 9 + 8
+    assert lib.tj_expert_plan_ints(32, 2, 8) == 9 + 128 + 8
+    assert lib.tj_expert_plan_ints(33, 2, 8) == 9 + 132 + 16
+    assert lib.tj_expert_plan_ints(100000, 4, 64) == 65 + 800000 + 148 * 64
+    assert lib.tj_expert_plan_ints(-1, 2, 8) == 0 and lib.tj_expert_plan_ints(1, 0, 8) == 0
+    assert lib.tj_expert_ffn_workspace_bytes(10, 2, 64, 128) == 20 * 256 + 20 * 128
+    assert lib.tj_expert_ffn_workspace_bytes(10, 0, 64, 128) == 0
+
+
+@pytest.mark.parametrize("kw,error", [
+    (dict(logits=torch.zeros(4, 8, dtype=torch.float64)), TypeError),
+    (dict(logits=torch.zeros(4)), ValueError),
+    (dict(logits=torch.zeros(8, 4).t()), ValueError),
+    (dict(top_k=0), ValueError),
+    (dict(top_k=9), ValueError),
+    (dict(logits=torch.zeros(4, 64), top_k=33), ValueError),
+    (dict(scoring="max"), ValueError),
+    (dict(bias=torch.zeros(7)), ValueError),
+    (dict(bias=torch.zeros(8, dtype=F16)), TypeError),
+    (dict(row_count=torch.zeros(2, dtype=I32)), ValueError),
+    (dict(row_count=torch.zeros(1, dtype=torch.int64)), TypeError),
+    (dict(logits=torch.zeros(4, 8, requires_grad=True)), RuntimeError),
+])
+def test_route_refusals(k, kw, error):
+    args = dict(logits=torch.zeros(4, 8), top_k=2)
+    with pytest.raises(_Unreached):
+        k.route_experts(**args)
+    args.update(kw)
+    with pytest.raises(error):
+        k.route_experts(**args)
+
+
+def test_no_grad_is_allowed(k):
+    with torch.no_grad(), pytest.raises(_Unreached):
+        k.route_experts(torch.zeros(4, 8, requires_grad=True), 2)
+
+
+def _routing(k, rows=4, top_k=2, E=3):
+    return k.ExpertRouting(torch.zeros(rows, top_k, dtype=I32), torch.zeros(rows, top_k),
+                           torch.zeros(E + 1 + 3 * rows * top_k, dtype=I32), E)
+
+
+@pytest.mark.parametrize("args,error", [
+    ((torch.zeros(4, 2), torch.zeros(4, 2), 3), TypeError),
+    ((torch.zeros(4, dtype=I32), torch.zeros(4), 3), ValueError),
+    ((torch.zeros(4, 33, dtype=I32), torch.zeros(4, 33), 3), ValueError),
+    ((torch.zeros(4, 2, dtype=I32), torch.zeros(4, 1), 3), ValueError),
+    ((torch.zeros(4, 2, dtype=I32), torch.zeros(4, 2), 0), ValueError),
+    ((torch.zeros(4, 2, dtype=I32), torch.zeros(4, 2), 513), ValueError),
+])
+def test_plan_refusals(k, args, error):
+    with pytest.raises(error):
+        k.expert_plan(*args)
+
+
+@pytest.mark.parametrize("kw,error", [
+    (dict(a=torch.zeros(4, 16)), TypeError),
+    (dict(a=torch.zeros(5, 16, dtype=F16)), ValueError),
+    (dict(a=torch.zeros(4, 24, dtype=F16)), ValueError),
+    (dict(w_in=torch.zeros(3, 32, 16, dtype=torch.bfloat16)), TypeError),
+    (dict(w_in=torch.zeros(2, 32, 16, dtype=F16)), ValueError),
+    (dict(w_out=torch.zeros(3, 16, 24, dtype=F16)), ValueError),
+    (dict(w_out=torch.zeros(3, 32, 16, dtype=F16).transpose(1, 2)), ValueError),
+    (dict(b_in=torch.zeros(3, 16)), ValueError),
+    (dict(b_out=torch.zeros(3, 16, dtype=F16)), TypeError),
+    (dict(routing=None), TypeError),
+    (dict(w_in=torch.zeros(3, 32, 16, dtype=F16, requires_grad=True)), RuntimeError),
+])
+def test_ffn_refusals(k, kw, error):
+    args = dict(a=torch.zeros(4, 16, dtype=F16), w_in=torch.zeros(3, 32, 16, dtype=F16), b_in=torch.zeros(3, 32),
+                w_out=torch.zeros(3, 16, 32, dtype=F16), b_out=None, routing=_routing(k))
+    with pytest.raises(_Unreached):
+        k.expert_ffn(**args)
+    args.update(kw)
+    with pytest.raises(error):
+        k.expert_ffn(**args)
+
+
+def test_gemm_and_combine_refusals(k):
+    r = _routing(k)
+    w = torch.zeros(3, 32, 16, dtype=F16)
+    for a, gather in ((torch.zeros(4, 16, dtype=F16), True), (torch.zeros(8, 16, dtype=F16), False)):
+        with pytest.raises(_Unreached):
+            k.gemm_experts(a, w, None, r, gather=gather)
+        with pytest.raises(ValueError):
+            k.gemm_experts(a, w, None, r, gather=not gather)
+        with pytest.raises(ValueError):
+            k.gemm_experts(a, w, torch.zeros(3, 16), r, gather=gather)
+    with pytest.raises(_Unreached):
+        k.expert_combine(torch.zeros(8, 16, dtype=F16), r)
+    with pytest.raises(ValueError):
+        k.expert_combine(torch.zeros(4, 16, dtype=F16), r)
+    with pytest.raises(TypeError):
+        k.expert_combine(torch.zeros(8, 16), r)
+    with pytest.raises(TypeError):
+        k.expert_combine(torch.zeros(8, 16, dtype=F16), object())
+
+
+@pytest.mark.parametrize("kw,error", [
+    (dict(x=torch.zeros(4, 16, dtype=F16)), TypeError),
+    (dict(x=torch.zeros(3, 16)), ValueError),
+    (dict(x=torch.zeros(64)), ValueError),
+    (dict(branch=torch.zeros(4, 16)), TypeError),
+    (dict(branch=torch.zeros(4, 8, dtype=F16)), ValueError),
+    (dict(pre_gamma=torch.ones(8)), ValueError),
+    (dict(pre_gamma=None), ValueError),
+    (dict(pre_beta=torch.ones(16, dtype=F16)), TypeError),
+    (dict(post_beta=torch.ones(16)), ValueError),
+    (dict(kind="batch"), ValueError),
+    (dict(gate_act="relu"), ValueError),
+    (dict(gate=torch.zeros(8)), ValueError),
+    (dict(gate=torch.zeros(16, dtype=F16)), TypeError),
+    (dict(gate=torch.zeros(4, 16, dtype=torch.bfloat16)), TypeError),
+    (dict(gate=torch.zeros(0, 16)), ValueError),
+    (dict(gate=torch.zeros(1, 16), rows_per_gate=3), ValueError),
+    (dict(gate=torch.zeros(4, 16), rows_per_gate=0), ValueError),
+    (dict(gate=torch.zeros(4, 16), gate_map=torch.zeros(3, dtype=I32)), ValueError),
+    (dict(row_map=torch.zeros(4)), TypeError),
+    (dict(row_map=torch.zeros(5, dtype=I32)), ValueError),
+    (dict(routing="r"), TypeError),
+    (dict(gate=torch.zeros(16, requires_grad=True)), RuntimeError),
+])
+def test_sandwich_refusals(k, kw, error):
+    args = dict(x=torch.zeros(4, 16), branch=torch.zeros(4, 16, dtype=F16), pre_gamma=torch.ones(16))
+    with pytest.raises(_Unreached):
+        k.sandwich_norm(**args)
+    args.update(kw)
+    with pytest.raises(error):
+        k.sandwich_norm(**args)
