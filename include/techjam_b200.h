@@ -298,6 +298,10 @@ TJ_API int tj_route_experts(const void* logits, int dtype, int rows, const int32
 TJ_API int tj_expert_plan(const int32_t* experts, int rows, int top_k, const int32_t* row_count,
                    int num_experts, int32_t* plan, void* stream);
 
+/* Workspace bytes tj_gemm_experts needs (0: none): gathered products of many
+ * rows per expert read a copy of a permuted to slot order. */
+TJ_API int64_t tj_gemm_experts_workspace_bytes(int rows, int top_k, int num_experts, int k, int gathered);
+
 /* out[s] = act(w[e] a[r] + bias[e]) for every slot s of the plan, e its expert
  * and r = its row (gathered != 0: a is [rows, k]) or s (a is [rows*top_k, k]);
  * act is erf-GELU on the fp32 sum if gelu != 0, else nothing.  out is
@@ -305,7 +309,7 @@ TJ_API int tj_expert_plan(const int32_t* experts, int rows, int top_k, const int
  * k multiples of 8, pointers 16-byte aligned, bias may be NULL. */
 TJ_API int tj_gemm_experts(const void* a, int dtype, int gathered, const void* w, const float* bias,
                     const int32_t* plan, int rows, int top_k, int num_experts, int n, int k, int gelu,
-                    void* out, void* stream);
+                    void* out, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* out[r] = sum over j of weights[r, j] * y[slot(r, j)], summed in fp32 and
  * rounded once; zeros for a row without experts.  Rows at or past *row_count
@@ -315,7 +319,7 @@ TJ_API int tj_expert_combine(const void* y, int dtype, const float* weights, con
                       void* out, void* stream);
 
 /* Workspace bytes tj_expert_ffn needs (0 on bad arguments). */
-TJ_API int64_t tj_expert_ffn_workspace_bytes(int rows, int top_k, int d_model, int ffn_dim);
+TJ_API int64_t tj_expert_ffn_workspace_bytes(int rows, int top_k, int num_experts, int d_model, int ffn_dim);
 
 /* out [rows, d_model] = the routed feed-forward of a [rows, d_model]:
  * w_in [E, ffn_dim, d_model], w_out [E, d_model, ffn_dim]; the hidden layer

@@ -189,10 +189,11 @@ SIGNATURES = {
     "tj_expert_plan": (c_int, [c_vp, c_int, c_int, c_vp, c_int, c_vp, c_vp]),
     "tj_gemm_experts": (
         c_int,
-        [c_vp, c_int, c_int, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int, c_int, c_vp, c_vp],
+        [c_vp, c_int, c_int, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int, c_int, c_vp, c_vp, c_i64, c_vp],
     ),
+    "tj_gemm_experts_workspace_bytes": (c_i64, [c_int, c_int, c_int, c_int, c_int]),
     "tj_expert_combine": (c_int, [c_vp, c_int, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_vp, c_vp]),
-    "tj_expert_ffn_workspace_bytes": (c_i64, [c_int, c_int, c_int, c_int]),
+    "tj_expert_ffn_workspace_bytes": (c_i64, [c_int, c_int, c_int, c_int, c_int]),
     "tj_expert_ffn": (
         c_int,
         [

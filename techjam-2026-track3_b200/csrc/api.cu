@@ -438,9 +438,14 @@ static int check_expert_shape(const char* what, int rows, int top_k, int num_exp
   return TJ_OK;
 }
 
+int64_t tj_gemm_experts_workspace_bytes(int rows, int top_k, int num_experts, int k, int gathered) {
+  if (rows < 0 || top_k < 1 || num_experts < 1 || k <= 0) return 0;
+  return experts_gemm_workspace((int64_t)rows * top_k, num_experts, k, gathered);
+}
+
 int tj_gemm_experts(const void* a, int dtype, int gathered, const void* w, const float* bias,
                     const int32_t* plan, int rows, int top_k, int num_experts, int n, int k, int gelu,
-                    void* out, void* stream) {
+                    void* out, void* workspace, int64_t workspace_bytes, void* stream) {
   int rc = check_device();
   if (rc) return rc;
   rc = check_expert_shape("gemm_experts", rows, top_k, num_experts);
@@ -461,6 +466,8 @@ int tj_gemm_experts(const void* a, int dtype, int gathered, const void* w, const
   g.N = n;
   g.K = k;
   g.out = out;
+  g.workspace = workspace;
+  g.workspace_bytes = workspace_bytes;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return finish(launch_experts_gemm(g, s), s);
 }
@@ -479,8 +486,10 @@ int tj_expert_combine(const void* y, int dtype, const float* weights, const int3
                 s);
 }
 
-int64_t tj_expert_ffn_workspace_bytes(int rows, int top_k, int d_model, int ffn_dim) {
-  if (rows < 0 || top_k < 1 || d_model <= 0 || ffn_dim <= 0) return 0;
+// h16 [slots, ffn_dim]; then, not needed at the same time, the permuted input
+// of FFN-in and the experts' outputs [slots, d_model].
+int64_t tj_expert_ffn_workspace_bytes(int rows, int top_k, int num_experts, int d_model, int ffn_dim) {
+  if (rows < 0 || top_k < 1 || num_experts < 1 || d_model <= 0 || ffn_dim <= 0) return 0;
   const size_t slots = (size_t)rows * top_k;
   return (int64_t)(align_up(slots * ffn_dim * 2, 256) + align_up(slots * d_model * 2, 256));
 }
@@ -497,7 +506,7 @@ int tj_expert_ffn(const void* a, int dtype, const void* w_in, const float* b_in,
     return set_error(TJ_ERR_UNSUPPORTED, "expert_ffn: d_model=%d and ffn_dim=%d must be multiples of 8", d_model, ffn_dim);
   if (!plan) return set_error(TJ_ERR_INVALID_ARGUMENT, "expert_ffn: null plan");
   if (rows == 0) return TJ_OK;
-  const int64_t need = tj_expert_ffn_workspace_bytes(rows, top_k, d_model, ffn_dim);
+  const int64_t need = tj_expert_ffn_workspace_bytes(rows, top_k, num_experts, d_model, ffn_dim);
   if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u))
     return set_error(TJ_ERR_WORKSPACE, "expert_ffn: workspace of %lld bytes (256-byte aligned), %lld needed",
                      (long long)workspace_bytes, (long long)need);
@@ -521,6 +530,8 @@ int tj_expert_ffn(const void* a, int dtype, const void* w_in, const float* b_in,
   g.N = ffn_dim;
   g.K = d_model;
   g.out = h16;
+  g.workspace = y16;
+  g.workspace_bytes = (int64_t)slots * d_model * 2;
   rc = launch_experts_gemm(g, s);
   if (rc) return rc;
   g.a = h16;

@@ -9,15 +9,21 @@
 // token costs one 16-column MMA per K step next to the weight bytes it has to
 // wait for.  The bias is one register per thread (thread = feature).
 //
-// One persistent CTA per SM, warps by role:
-//   warp 0      weight tiles [128 features x 64] by TMA
-//   warp 1      token tiles [up to BN rows x 64]: FFN-in gathers the rows of the
-//               slots' tokens with TMA row gathers (4 rows per instruction, the
-//               lanes issue in parallel), so no permuted copy of the activations
-//               exists; FFN-out reads consecutive slots
-//   warp 2      TMEM allocation and tcgen05.mma (M=128, N=16..BN, K=16)
-//   warps 4-11  epilogue: TMEM -> bias, GELU -> 16 bits -> shared memory
-//               transposed to [token][feature] -> 256-byte rows of `out`
+// Persistent CTAs, one per SM, warps by role:
+//   warp 0       weight tiles [128 features x 64] by TMA
+//   warp 1       token tiles [tokens x 64] by TMA: consecutive slots, or the
+//                rows of the slots' tokens (TMA row gather, 4 rows per instruction)
+//   warp 2       TMEM allocation and tcgen05.mma (K=16 per instruction)
+//   warps 4-11   epilogue: TMEM -> bias, GELU -> 16 bits -> shared memory
+//                transposed to [token][feature] -> 256-byte rows of `out`
+// With many tokens per expert two CTAs form a pair (tcgen05 cta_group::2): 256
+// features x up to 256 tokens, each CTA loading half of either operand, 32 KB
+// per K step of 64 instead of 48 KB; both CTAs' loads arrive on the leader's
+// barrier, as in the dense GEMM.  Pairs read consecutive slots only: a row
+// gather takes 73 cycles of the TMA unit, and cp.async gathers wait for a
+// proxy fence (about 1800 cycles with copies in flight) per stage.  48002
+// slots, D 1024, F 4096: 1590 us by TMA gathers, 620 us by cp.async, 310 us
+// from a permuted copy, which expert_gather_kernel writes in about 30 us.
 // Two accumulators overlap a tile's epilogue with the next tile's products.
 // Every CTA reads the plan's offsets and derives the tile list itself: the
 // host never learns the counts.
@@ -30,14 +36,18 @@ constexpr int kXpThreads = 384;
 constexpr int kXpEpiWarps = 8;
 constexpr uint32_t kXpScratchBytes = 2 * 32 * 256;  // per epilogue group: 32 tokens x 128 features
 
-template <int BN>
+// BN: tokens of a tile; with kPair half of them in each CTA.
+template <bool kPair, int BN>
 struct XpCfg {
-  static constexpr int kStages = BN >= 256 ? 4 : 9;
+  static constexpr int kXRows = kPair ? BN / 2 : BN;         // token rows of this CTA
+  static constexpr int kFeatures = kPair ? 2 * kBM : kBM;    // of a tile
+  static constexpr int kStages = kPair ? 6 : (BN >= 64 ? 7 : 9);
   static constexpr uint32_t kWBytes = kBM * kBK * 2;
-  static constexpr uint32_t kXBytes = BN * kBK * 2;
+  static constexpr uint32_t kXBytes = kXRows * kBK * 2;
   static constexpr uint32_t kStageBytes = kWBytes + kXBytes;
-  static constexpr uint32_t kTmemCols = 2 * BN < 32 ? 32 : 2 * BN;
-  static constexpr int kBoxRows = 32;  // rows of one token load (FFN-out)
+  static constexpr uint32_t kTmemCols = 2 * BN;
+  static constexpr int kStep = kPair ? 32 : 16;              // tokens of a tile: a multiple of this
+  static constexpr int kBoxRows = 32;                        // rows of one token load
   static constexpr size_t smem_bytes(int experts) {
     return 1024 + (size_t)kStages * kStageBytes + kXpScratchBytes + 512 + (size_t)(2 * experts + 2) * sizeof(int);
   }
@@ -50,6 +60,15 @@ struct XpParams {
   void* out;                // [slots][N]
   int slots, rows, E, N, K;
 };
+
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, uint32_t cluster_bar, int c0,
+                                                 int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(cluster_bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
 
 __device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int r0, int r1,
                                             int r2, int r3) {
@@ -83,8 +102,8 @@ struct XpTile {
 
 // Walks the tiles of all experts in order.  first[e]: first slot of expert e;
 // tiles[e]: first tile of expert e (tiles[E] = total).  An expert's tokens are
-// cut into equal tiles of a multiple of 16 tokens, at most BN.
-template <int BN>
+// cut into equal tiles of a multiple of kStep tokens, at most BN.
+template <int BN, int kStep, int kFeatures>
 struct XpWalk {
   const int* first;
   const int* tiles;
@@ -95,31 +114,31 @@ struct XpWalk {
     while (t >= tiles[e + 1]) ++e;
     const int n = first[e + 1] - first[e];
     const int cuts = (n + BN - 1) / BN;
-    const int size = ((n + cuts - 1) / cuts + 15) & ~15;
+    const int size = ((n + cuts - 1) / cuts + kStep - 1) / kStep * kStep;
     const int local = t - tiles[e];
     const int cut = local / m_tiles;
     XpTile r;
     r.e = e;
     r.s0 = first[e] + cut * size;
     r.n = min(size, first[e + 1] - r.s0);
-    r.m0 = (local - cut * m_tiles) * kBM;
+    r.m0 = (local - cut * m_tiles) * kFeatures;
     return r;
   }
 };
 
-template <int BN, bool kGelu, bool kGather, typename T>
-__global__ void __launch_bounds__(kXpThreads, 1)
-    experts_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
-                        const XpParams p) {
-  using Cfg = XpCfg<BN>;
+template <bool kPair, int BN, bool kGelu, bool kGather, typename T>
+__device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const CUtensorMap& tmX, const XpParams& p) {
+  using Cfg = XpCfg<kPair, BN>;
+  using Walk = XpWalk<BN, Cfg::kStep, Cfg::kFeatures>;
   constexpr int S = Cfg::kStages;
+  constexpr int kCtas = kPair ? 2 : 1;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* sW = smem;
   uint8_t* sX = smem + S * Cfg::kWBytes;
   const uint32_t scratch = smem_u32(sX + S * Cfg::kXBytes);
   uint64_t* bars = reinterpret_cast<uint64_t*>(sX + S * Cfg::kXBytes + kXpScratchBytes);
-  // bars: full[S], empty[S], tfull[2], tempty[2], final
+  // bars: full[S] (leader's used), empty[S], tfull[2], tempty[2] (leader's used), final
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 5);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* first = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(bars) + 512);  // [E+1]
@@ -127,6 +146,8 @@ __global__ void __launch_bounds__(kXpThreads, 1)
 
   const int warp = warp_idx();
   const int lane = (int)lane_id();
+  const int rank = kPair ? (int)cluster_ctarank() : 0;
+  const bool leader = rank == 0;
   auto full_bar = [&](int s) { return smem_u32(bars + s); };
   auto empty_bar = [&](int s) { return smem_u32(bars + S + s); };
   auto tfull_bar = [&](int a) { return smem_u32(bars + 2 * S + a); };
@@ -140,7 +161,7 @@ __global__ void __launch_bounds__(kXpThreads, 1)
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(tfull_bar(a), 1);
-      mbar_init(tempty_bar(a), kXpEpiWarps);
+      mbar_init(tempty_bar(a), kCtas * kXpEpiWarps);
     }
     mbar_init(final_bar, 1);
     *abort_flag = device_failed() ? 1 : 0;
@@ -149,11 +170,16 @@ __global__ void __launch_bounds__(kXpThreads, 1)
     tma_prefetch_desc(&tmX);
   }
   if (warp == 2) {
-    tmem_alloc(smem_u32(tmem_slot), Cfg::kTmemCols);
-    tmem_relinquish();
+    if constexpr (kPair) {
+      tmem_alloc_pair(smem_u32(tmem_slot), Cfg::kTmemCols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(smem_u32(tmem_slot), Cfg::kTmemCols);
+      tmem_relinquish();
+    }
   }
   pdl_wait();
-  const int m_tiles = (p.N + kBM - 1) / kBM;
+  const int m_tiles = (p.N + Cfg::kFeatures - 1) / Cfg::kFeatures;
   // Offsets, held inside [0, slots] whatever the plan says.
   for (int e = threadIdx.x; e <= p.E; e += kXpThreads) {
     const int o = p.offsets[e];
@@ -173,24 +199,31 @@ __global__ void __launch_bounds__(kXpThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (kPair) cluster_sync();  // the peer's barriers are initialised
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const int total_tiles = tiles[p.E];
   const int k_blocks = (p.K + kBK - 1) / kBK;
+  const int tile0 = (int)blockIdx.x / kCtas;
+  const int tile_step = (int)gridDim.x / kCtas;
 
   if (warp == 0) {
     if (lane == 0) {
-      XpWalk<BN> walk(first, tiles, m_tiles);
+      Walk walk(first, tiles, m_tiles);
       int stage = 0;
       uint32_t phase = 0;
       int last_parity[S];
       for (int s = 0; s < S; ++s) last_parity[s] = -1;
-      for (int t = blockIdx.x; t < total_tiles && !*abort_flag; t += gridDim.x) {
+      for (int t = tile0; t < total_tiles && !*abort_flag; t += tile_step) {
         const XpTile tile = walk.at(t);
         for (int kb = 0; kb < k_blocks; ++kb) {
           if (!mbar_wait(empty_bar(stage), phase ^ 1, abort_flag, 250)) break;
-          mbar_arrive_expect_tx(full_bar(stage), Cfg::kWBytes);
-          tma_load_3d(smem_u32(sW + stage * Cfg::kWBytes), &tmW, full_bar(stage), kb * kBK, tile.m0, tile.e);
+          if (leader) mbar_arrive_expect_tx(full_bar(stage), kCtas * Cfg::kWBytes);
+          const uint32_t dst = smem_u32(sW + stage * Cfg::kWBytes);
+          if constexpr (kPair)
+            tma_load_3d_pair(dst, &tmW, mapa_shared(full_bar(stage), 0), kb * kBK, tile.m0 + rank * kBM, tile.e);
+          else
+            tma_load_3d(dst, &tmW, full_bar(stage), kb * kBK, tile.m0, tile.e);
           last_parity[stage] = (int)phase;
           if (++stage == S) {
             stage = 0;
@@ -198,52 +231,46 @@ __global__ void __launch_bounds__(kXpThreads, 1)
           }
         }
       }
-      // Both producers' loads have landed once the stage's barrier completes.
-      for (int s = 0; s < S; ++s)
-        if (last_parity[s] >= 0) drain_wait(full_bar(s), (uint32_t)last_parity[s]);
+      // Every load of both producers (and of the peer) has landed once the
+      // leader's barriers complete.
+      if (leader)
+        for (int s = 0; s < S; ++s)
+          if (last_parity[s] >= 0) drain_wait(full_bar(s), (uint32_t)last_parity[s]);
     }
   } else if (warp == 1) {
-    XpWalk<BN> walk(first, tiles, m_tiles);
+    Walk walk(first, tiles, m_tiles);
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < total_tiles && ok; t += gridDim.x) {
+    for (int t = tile0; t < total_tiles && ok; t += tile_step) {
       const XpTile tile = walk.at(t);
-      const int cols = (tile.n + 15) & ~15;
-      constexpr int kQuads = BN >= 128 ? BN / 128 : 1;  // 4-row gathers per lane
-      int row[kQuads][4];
+      const int cols = (tile.n + Cfg::kStep - 1) / Cfg::kStep * Cfg::kStep / kCtas;  // this CTA's
+      constexpr int kRows = kGather ? 4 : Cfg::kBoxRows;                             // of one load
+      const int loads = (cols + kRows - 1) / kRows;
+      int row[4] = {tile.s0 + rank * cols + lane * kRows, 0, 0, 0};
       if constexpr (kGather) {
 #pragma unroll
-        for (int q = 0; q < kQuads; ++q)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            // columns past the tile's tokens repeat its last one (never stored)
-            const int s = tile.s0 + min((q * 32 + lane) * 4 + i, tile.n - 1);
-            const int r = __ldg(p.slot_row + s);
-            if (r < 0 || r >= p.rows) report_error(kDevBadArgument, 245);
-            row[q][i] = min(max(r, 0), p.rows - 1);
-          }
+        for (int i = 0; i < 4; ++i) {
+          // columns past the tile's tokens repeat its last one (never stored)
+          const int r = __ldg(p.slot_row + tile.s0 + min(lane * 4 + i, tile.n - 1));
+          if (r < 0 || r >= p.rows) report_error(kDevBadArgument, 245);
+          row[i] = min(max(r, 0), p.rows - 1);
+        }
       }
-      const uint32_t bytes = kGather ? (uint32_t)cols * 128u
-                                     : (uint32_t)((cols + Cfg::kBoxRows - 1) / Cfg::kBoxRows) * Cfg::kBoxRows * 128u;
       for (int kb = 0; kb < k_blocks; ++kb) {
         ok = mbar_wait(empty_bar(stage), phase ^ 1, abort_flag, 251);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        const uint32_t dst = smem_u32(sX + stage * Cfg::kXBytes);
-        if (lane == 0) mbar_arrive_expect_tx(full_bar(stage), bytes);
+        const uint32_t dst = smem_u32(sX + stage * Cfg::kXBytes) + lane * (kRows * 128);
+        if (leader && lane == 0) mbar_arrive_expect_tx(full_bar(stage), (uint32_t)(kCtas * loads * kRows * 128));
         __syncwarp();
-        if constexpr (kGather) {
-#pragma unroll
-          for (int q = 0; q < kQuads; ++q) {
-            const int quad = q * 32 + lane;
-            if (quad * 4 < cols)
-              tma_gather4(dst + quad * 512, &tmX, full_bar(stage), kb * kBK, row[q][0], row[q][1], row[q][2], row[q][3]);
-          }
-        } else {
-          if (lane * Cfg::kBoxRows < cols)
-            tma_load_2d(dst + lane * Cfg::kBoxRows * 128, &tmX, full_bar(stage), kb * kBK,
-                        tile.s0 + lane * Cfg::kBoxRows);
+        if (lane < loads) {
+          if constexpr (kGather)
+            tma_gather4(dst, &tmX, full_bar(stage), kb * kBK, row[0], row[1], row[2], row[3]);
+          else if constexpr (kPair)
+            tma_load_2d_pair(dst, &tmX, mapa_shared(full_bar(stage), 0), kb * kBK, row[0]);
+          else
+            tma_load_2d(dst, &tmX, full_bar(stage), kb * kBK, row[0]);
         }
         if (++stage == S) {
           stage = 0;
@@ -252,22 +279,23 @@ __global__ void __launch_bounds__(kXpThreads, 1)
       }
     }
   } else if (warp == 2) {
-    if (lane == 0) {
-      XpWalk<BN> walk(first, tiles, m_tiles);
+    if (leader && lane == 0) {
+      Walk walk(first, tiles, m_tiles);
       int stage = 0;
       uint32_t phase = 0;
       int acc = 0;
       uint32_t acc_phase = 0;
       bool issued = false;
-      for (int t = blockIdx.x; t < total_tiles && !*abort_flag; t += gridDim.x) {
+      for (int t = tile0; t < total_tiles && !*abort_flag; t += tile_step) {
         const XpTile tile = walk.at(t);
-        const uint32_t idesc = idesc_f16_f32(kBM, (tile.n + 15) & ~15, 0, 0) | XpType<T>::kFormat;
-        if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1, abort_flag, 252)) break;
+        const int cols = (tile.n + Cfg::kStep - 1) / Cfg::kStep * Cfg::kStep;
+        const uint32_t idesc = idesc_f16_f32(Cfg::kFeatures, cols, 0, 0) | XpType<T>::kFormat;
+        if (!mbar_wait<kPair>(tempty_bar(acc), acc_phase ^ 1, abort_flag, 252)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
         bool ok = true;
         for (int kb = 0; kb < k_blocks; ++kb) {
-          if (!mbar_wait(full_bar(stage), phase, abort_flag, 253)) {
+          if (!mbar_wait<kPair>(full_bar(stage), phase, abort_flag, 253)) {
             ok = false;
             break;
           }
@@ -275,38 +303,57 @@ __global__ void __launch_bounds__(kXpThreads, 1)
           const uint64_t a_desc = sw128_desc(smem_u32(sW + stage * Cfg::kWBytes), 16, 1024);
           const uint64_t b_desc = sw128_desc(smem_u32(sX + stage * Cfg::kXBytes), 16, 1024);
 #pragma unroll
-          for (int k = 0; k < kBK / 16; ++k)
-            mma_f16_ss(d_tmem, a_desc + (uint64_t)(2 * k), b_desc + (uint64_t)(2 * k), idesc, (kb | k) != 0 ? 1u : 0u);
+          for (int k = 0; k < kBK / 16; ++k) {
+            const uint64_t ak = a_desc + (uint64_t)(2 * k), bk = b_desc + (uint64_t)(2 * k);
+            if constexpr (kPair)
+              mma_f16_ss_pair(d_tmem, ak, bk, idesc, (kb | k) != 0 ? 1u : 0u);
+            else
+              mma_f16_ss(d_tmem, ak, bk, idesc, (kb | k) != 0 ? 1u : 0u);
+          }
           issued = true;
-          mma_commit(empty_bar(stage));
+          if constexpr (kPair) {
+            mma_commit_pair(empty_bar(stage));
+            mma_commit_pair(mapa_shared(empty_bar(stage), 1));
+          } else {
+            mma_commit(empty_bar(stage));
+          }
           if (++stage == S) {
             stage = 0;
             phase ^= 1;
           }
         }
         if (!ok) break;
-        mma_commit(tfull_bar(acc));
+        if constexpr (kPair) {
+          mma_commit_pair(tfull_bar(acc));
+          mma_commit_pair(mapa_shared(tfull_bar(acc), 1));
+        } else {
+          mma_commit(tfull_bar(acc));
+        }
         if (++acc == 2) {
           acc = 0;
           acc_phase ^= 1;
         }
       }
       if (issued) {
-        mma_commit(final_bar);
+        if constexpr (kPair)
+          mma_commit_pair(final_bar);
+        else
+          mma_commit(final_bar);
         drain_wait(final_bar, 0);
       }
     }
   } else if (warp >= 4) {
-    XpWalk<BN> walk(first, tiles, m_tiles);
+    Walk walk(first, tiles, m_tiles);
     const int quarter = warp & 3;
     const int group = (warp - 4) >> 2;
-    const int tid = quarter * 32 + lane;  // feature inside the tile
+    const int tid = quarter * 32 + lane;  // feature inside this CTA's 128
     const uint32_t buf = scratch + (uint32_t)group * (kXpScratchBytes / 2);
     const int bar_id = 1 + group;
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int t = blockIdx.x; t < total_tiles; t += gridDim.x) {
-      const XpTile tile = walk.at(t);
+    for (int t = tile0; t < total_tiles; t += tile_step) {
+      XpTile tile = walk.at(t);
+      tile.m0 += rank * kBM;
       const float bias = (p.bias && tile.m0 + tid < p.N) ? __ldg(p.bias + (int64_t)tile.e * p.N + tile.m0 + tid) : 0.f;
       const bool ok = mbar_wait(tfull_bar(acc), acc_phase, abort_flag, 254);
       // The four warps of a group meet at barriers below, so they leave together.
@@ -338,7 +385,12 @@ __global__ void __launch_bounds__(kXpThreads, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_relaxed(tempty_bar(acc));
+      if (lane == 0) {
+        if constexpr (kPair)
+          mbar_arrive_cluster_relaxed(mapa_shared(tempty_bar(acc), 0));
+        else
+          mbar_arrive_relaxed(tempty_bar(acc));
+      }
       if (++acc == 2) {
         acc = 0;
         acc_phase ^= 1;
@@ -349,16 +401,71 @@ __global__ void __launch_bounds__(kXpThreads, 1)
   __syncwarp();
   pdl_trigger();
   tc_fence_before();
-  __syncthreads();
+  if constexpr (kPair)
+    cluster_sync();  // the peer no longer reads this CTA's shared memory or barriers
+  else
+    __syncthreads();
   if (warp == 2) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, Cfg::kTmemCols);
+    if constexpr (kPair)
+      tmem_dealloc_pair(tmem_base, Cfg::kTmemCols);
+    else
+      tmem_dealloc(tmem_base, Cfg::kTmemCols);
   }
 }
 
 template <int BN, bool kGelu, bool kGather, typename T>
+__global__ void __launch_bounds__(kXpThreads, 1)
+    experts_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                        const XpParams p) {
+  experts_gemm_body<false, BN, kGelu, kGather, T>(tmW, tmX, p);
+}
+
+template <int BN, bool kGelu, typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kXpThreads, 1)
+    experts_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                             const XpParams p) {
+  experts_gemm_body<true, BN, kGelu, false, T>(tmW, tmX, p);
+}
+
+// CTAs to launch at most: one per SM, for pairs as many as fit in clusters.
+template <bool kPair, int BN, bool kGelu, bool kGather, typename T>
+static int experts_gemm_ctas(int* ctas) {
+  using Cfg = XpCfg<kPair, BN>;
+  int num_sms = 0;
+  int rc = ensure_device_props(&num_sms);
+  if (rc) return rc;
+  static int cache[64] = {};
+  int& cached = cache[device_index()];
+  if (cached == 0) {
+    void (*kernel)(CUtensorMap, CUtensorMap, XpParams);
+    if constexpr (kPair)
+      kernel = experts_gemm_pair_kernel<BN, kGelu, T>;
+    else
+      kernel = experts_gemm_kernel<BN, kGelu, kGather, T>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)Cfg::smem_bytes(kRouteMaxExperts));
+    if (e != cudaSuccess) return set_error(TJ_ERR_CUDA, "gemm_experts smem attribute: %s", cudaGetErrorString(e));
+    int n = num_sms;
+    if (kPair) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(num_sms & ~1);
+      cfg.blockDim = dim3(kXpThreads);
+      cfg.dynamicSmemBytes = Cfg::smem_bytes(kRouteMaxExperts);
+      e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+      if (e != cudaSuccess) return set_error(TJ_ERR_CUDA, "gemm_experts occupancy: %s", cudaGetErrorString(e));
+      n *= 2;
+    }
+    if (n <= 0) return set_error(TJ_ERR_UNSUPPORTED, "gemm_experts: the kernel does not fit this device");
+    cached = n;
+  }
+  *ctas = cached;
+  return TJ_OK;
+}
+
+template <bool kPair, int BN, bool kGelu, bool kGather, typename T>
 static int launch_experts_gemm_t(const ExpertGemmArgs& a, const XpParams& kp, cudaStream_t stream) {
-  using Cfg = XpCfg<BN>;
+  using Cfg = XpCfg<kPair, BN>;
   CUtensorMap tw, tx;
   uint64_t dw[3] = {(uint64_t)a.K, (uint64_t)a.N, (uint64_t)a.num_experts};
   uint64_t sw[2] = {(uint64_t)a.K, (uint64_t)a.K * (uint64_t)a.N};
@@ -370,44 +477,89 @@ static int launch_experts_gemm_t(const ExpertGemmArgs& a, const XpParams& kp, cu
   uint32_t bx[2] = {kBK, kGather ? 1u : (uint32_t)Cfg::kBoxRows};
   rc = make_tmap_f16(&tx, a.a, 2, dx, sx, bx);
   if (rc) return rc;
-  int num_sms = 0;
-  rc = ensure_device_props(&num_sms);
+  int ctas = 0;
+  rc = experts_gemm_ctas<kPair, BN, kGelu, kGather, T>(&ctas);
   if (rc) return rc;
-  auto* kernel = experts_gemm_kernel<BN, kGelu, kGather, T>;
-  static bool attr_set[64] = {};
-  const int dev = device_index();
-  if (!attr_set[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)Cfg::smem_bytes(kRouteMaxExperts));
-    if (e != cudaSuccess) return set_error(TJ_ERR_CUDA, "gemm_experts smem attribute: %s", cudaGetErrorString(e));
-    attr_set[dev] = true;
-  }
-  const int64_t m_tiles = (a.N + kBM - 1) / kBM;
+  const int64_t m_tiles = (a.N + Cfg::kFeatures - 1) / Cfg::kFeatures;
   const int64_t reached = a.slots < a.num_experts ? a.slots : a.num_experts;
   const int64_t max_tiles = (a.slots / BN + reached) * m_tiles;
   if (max_tiles > INT32_MAX) return set_error(TJ_ERR_UNSUPPORTED, "gemm_experts: too many tiles");
-  const int grid = (int)(max_tiles < num_sms ? max_tiles : num_sms);
-  cudaError_t e = launch_pdl(kernel, dim3(grid), dim3(kXpThreads), Cfg::smem_bytes(a.num_experts), stream, tw, tx, kp);
+  const int64_t want = max_tiles * (kPair ? 2 : 1);
+  const int grid = (int)(want < ctas ? want : ctas);
+  cudaError_t e;
+  if constexpr (kPair)
+    e = launch_pdl(experts_gemm_pair_kernel<BN, kGelu, T>, dim3(grid), dim3(kXpThreads),
+                   Cfg::smem_bytes(a.num_experts), stream, tw, tx, kp);
+  else
+    e = launch_pdl(experts_gemm_kernel<BN, kGelu, kGather, T>, dim3(grid), dim3(kXpThreads),
+                   Cfg::smem_bytes(a.num_experts), stream, tw, tx, kp);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(TJ_ERR_CUDA, "gemm_experts launch: %s", cudaGetErrorString(e));
   return TJ_OK;
 }
 
-template <int BN>
+template <bool kPair, int BN, bool kGather>
 static int launch_experts_gemm_bn(const ExpertGemmArgs& a, const XpParams& kp, cudaStream_t stream) {
   const bool bf16 = a.dtype == TJ_DTYPE_BF16;
-  if (a.gather) {
-    if (a.gelu)
-      return bf16 ? launch_experts_gemm_t<BN, true, true, __nv_bfloat16>(a, kp, stream)
-                  : launch_experts_gemm_t<BN, true, true, __half>(a, kp, stream);
-    return bf16 ? launch_experts_gemm_t<BN, false, true, __nv_bfloat16>(a, kp, stream)
-                : launch_experts_gemm_t<BN, false, true, __half>(a, kp, stream);
-  }
   if (a.gelu)
-    return bf16 ? launch_experts_gemm_t<BN, true, false, __nv_bfloat16>(a, kp, stream)
-                : launch_experts_gemm_t<BN, true, false, __half>(a, kp, stream);
-  return bf16 ? launch_experts_gemm_t<BN, false, false, __nv_bfloat16>(a, kp, stream)
-              : launch_experts_gemm_t<BN, false, false, __half>(a, kp, stream);
+    return bf16 ? launch_experts_gemm_t<kPair, BN, true, kGather, __nv_bfloat16>(a, kp, stream)
+                : launch_experts_gemm_t<kPair, BN, true, kGather, __half>(a, kp, stream);
+  return bf16 ? launch_experts_gemm_t<kPair, BN, false, kGather, __nv_bfloat16>(a, kp, stream)
+              : launch_experts_gemm_t<kPair, BN, false, kGather, __half>(a, kp, stream);
+}
+
+// Permuted copy: out[s] = a[slot_row[s]] for the plan's slots, 16 bytes a
+// thread (rows are whole 16-byte units).  Reads and writes each byte once; what
+// it writes stays in L2 for the products that follow, as far as it fits.
+__global__ void __launch_bounds__(256) expert_gather_kernel(const uint4* __restrict__ a,
+                                                            const int32_t* __restrict__ offsets,
+                                                            const int32_t* __restrict__ slot_row, int slots, int rows,
+                                                            int E, int units, uint4* __restrict__ out) {
+  pdl_wait();
+  pdl_trigger();
+  const int used = min(max(offsets[E], 0), slots);
+  const int64_t n = (int64_t)used * units;
+  const int64_t step = (int64_t)gridDim.x * 256;
+  int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  constexpr int kFlight = 4;  // loads in flight per thread
+  for (; i < n; i += kFlight * step) {
+    uint4 v[kFlight];
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u) {
+      const int64_t j = i + u * step;
+      if (j < n) {
+        const int s = (int)(j / units);
+        const int r = __ldg(slot_row + s);
+        if (r < 0 || r >= rows) report_error(kDevBadArgument, 246);
+        v[u] = __ldg(a + (int64_t)min(max(r, 0), rows - 1) * units + (j - (int64_t)s * units));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u)
+      if (i + u * step < n) out[i + u * step] = v[u];
+  }
+}
+
+static int launch_expert_gather(const ExpertGemmArgs& a, void* out, cudaStream_t stream) {
+  const int units = a.K / 8;
+  int num_sms = 0;
+  int rc = ensure_device_props(&num_sms);
+  if (rc) return rc;
+  const int64_t blocks = ((int64_t)a.slots * units + 1023) / 1024;
+  const int grid = (int)(blocks < 8 * num_sms ? blocks : 8 * num_sms);
+  cudaError_t e = launch_pdl(expert_gather_kernel, dim3(grid), dim3(256), 0, stream, static_cast<const uint4*>(a.a),
+                             a.offsets, a.slot_row, a.slots, a.a_rows, a.num_experts, units, static_cast<uint4*>(out));
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return set_error(TJ_ERR_CUDA, "expert_gather launch: %s", cudaGetErrorString(e));
+  return TJ_OK;
+}
+
+// Pairs of CTAs with tiles of up to 256 tokens once the experts have more than
+// 32 on average, else one CTA with tiles of up to 32.
+static bool experts_gemm_pairs(int64_t slots, int num_experts) { return slots > 32 * (int64_t)num_experts; }
+
+int64_t experts_gemm_workspace(int64_t slots, int num_experts, int k, int gather) {
+  return gather && experts_gemm_pairs(slots, num_experts) ? slots * k * 2 : 0;
 }
 
 int launch_experts_gemm(const ExpertGemmArgs& a, cudaStream_t stream) {
@@ -437,9 +589,22 @@ int launch_experts_gemm(const ExpertGemmArgs& a, cudaStream_t stream) {
   kp.E = a.num_experts;
   kp.N = a.N;
   kp.K = a.K;
-  // Tiles of 256 tokens once the experts have more than 32 on average.
-  if (a.slots > 32 * a.num_experts) return launch_experts_gemm_bn<256>(a, kp, stream);
-  return launch_experts_gemm_bn<32>(a, kp, stream);
+  if (experts_gemm_pairs(a.slots, a.num_experts)) {
+    ExpertGemmArgs g = a;
+    if (a.gather) {
+      if (!a.workspace || a.workspace_bytes < experts_gemm_workspace(a.slots, a.num_experts, a.K, 1) ||
+          (reinterpret_cast<uintptr_t>(a.workspace) & 15u))
+        return set_error(TJ_ERR_WORKSPACE, "gemm_experts: workspace of %lld bytes (16-byte aligned), %lld needed",
+                         (long long)a.workspace_bytes, (long long)a.slots * a.K * 2);
+      int rc = launch_expert_gather(a, a.workspace, stream);
+      if (rc) return rc;
+      g.a = a.workspace;
+      g.a_rows = a.slots;
+    }
+    return launch_experts_gemm_bn<true, 256, false>(g, kp, stream);
+  }
+  if (a.gather) return launch_experts_gemm_bn<false, 32, true>(a, kp, stream);
+  return launch_experts_gemm_bn<false, 32, false>(a, kp, stream);
 }
 
 }  // namespace tj

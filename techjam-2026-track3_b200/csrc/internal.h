@@ -165,7 +165,10 @@ struct ExpertGemmArgs {
   int dtype, gather, gelu;
   int slots, a_rows, num_experts, N, K;
   void* out;                // [slots][N]
+  void* workspace;          // gather: experts_gemm_workspace bytes
+  int64_t workspace_bytes;
 };
+int64_t experts_gemm_workspace(int64_t slots, int num_experts, int k, int gather);
 int launch_experts_gemm(const ExpertGemmArgs& args, cudaStream_t stream);
 
 int launch_expert_combine(int dtype, const void* y, const float* weights, const int32_t* row_slot,

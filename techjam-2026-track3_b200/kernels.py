@@ -533,9 +533,11 @@ def gemm_experts(a, w, bias, routing, *, gather, gelu=False, out=None):
         if out is None:
             out = torch.empty(slots, N, dtype=a.dtype, device=dev)
         _require_out(out, "out", (slots, N), a.dtype, dev)
+        need = lib.tj_gemm_experts_workspace_bytes(routing.rows, routing.top_k, routing.num_experts, K, 1 if gather else 0)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         rc = lib.tj_gemm_experts(
             a.data_ptr(), code, 1 if gather else 0, w.data_ptr(), _ptr(bias), routing.plan.data_ptr(), routing.rows,
-            routing.top_k, routing.num_experts, N, K, 1 if gelu else 0, out.data_ptr(), _stream(a),
+            routing.top_k, routing.num_experts, N, K, 1 if gelu else 0, out.data_ptr(), _ptr(ws), need, _stream(a),
         )
     _lib.check(rc, "gemm_experts")
     return out
@@ -594,7 +596,7 @@ def expert_ffn(a, w_in, b_in, w_out, b_out, routing, *, out=None):
         if out is None:
             out = torch.empty(routing.rows, D, dtype=a.dtype, device=dev)
         _require_out(out, "out", (routing.rows, D), a.dtype, dev)
-        need = lib.tj_expert_ffn_workspace_bytes(routing.rows, routing.top_k, D, F)
+        need = lib.tj_expert_ffn_workspace_bytes(routing.rows, routing.top_k, E, D, F)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
         rc = lib.tj_expert_ffn(
             a.data_ptr(), code, w_in.data_ptr(), _ptr(b_in), w_out.data_ptr(), _ptr(b_out),
