@@ -323,7 +323,8 @@ TJ_API int64_t tj_expert_ffn_workspace_bytes(int rows, int top_k, int num_expert
 
 /* out [rows, d_model] = the routed feed-forward of a [rows, d_model]:
  * w_in [E, ffn_dim, d_model], w_out [E, d_model, ffn_dim]; the hidden layer
- * and each expert's output are rounded to `dtype` once, as the dense FFN's. */
+ * is rounded to `dtype` once, the experts' outputs stay fp32 until their sum
+ * is. */
 TJ_API int tj_expert_ffn(const void* a, int dtype, const void* w_in, const float* b_in, const void* w_out,
                   const float* b_out, const float* weights, const int32_t* plan,
                   const int32_t* row_count, int rows, int top_k, int num_experts, int d_model,

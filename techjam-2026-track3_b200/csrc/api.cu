@@ -481,17 +481,22 @@ int tj_expert_combine(const void* y, int dtype, const float* weights, const int3
   if (rc) return rc;
   if (!plan) return set_error(TJ_ERR_INVALID_ARGUMENT, "expert_combine: null plan");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return finish(launch_expert_combine(dtype, y, weights, plan_row_slot(plan, num_experts, rows, top_k), row_count,
+  return finish(launch_expert_combine(dtype, 0, y, weights, plan_row_slot(plan, num_experts, rows, top_k), row_count,
                                       rows, top_k, d_model, out, s),
                 s);
 }
 
-// h16 [slots, ffn_dim]; then, not needed at the same time, the permuted input
-// of FFN-in and the experts' outputs [slots, d_model].
+// Experts' outputs in fp32 planes; before they are written, the permuted input
+// of FFN-in lies in the same place.
+static size_t expert_ffn_out_bytes(int64_t slots, int num_experts, int d_model, int ffn_dim) {
+  return (size_t)slots * d_model * 4 * experts_gemm_splits(slots, num_experts, d_model, ffn_dim);
+}
+
 int64_t tj_expert_ffn_workspace_bytes(int rows, int top_k, int num_experts, int d_model, int ffn_dim) {
   if (rows < 0 || top_k < 1 || num_experts < 1 || d_model <= 0 || ffn_dim <= 0) return 0;
-  const size_t slots = (size_t)rows * top_k;
-  return (int64_t)(align_up(slots * ffn_dim * 2, 256) + align_up(slots * d_model * 2, 256));
+  const int64_t slots = (int64_t)rows * top_k;
+  return (int64_t)(align_up((size_t)slots * ffn_dim * 2, 256) +
+                   align_up(expert_ffn_out_bytes(slots, num_experts, d_model, ffn_dim), 256));
 }
 
 int tj_expert_ffn(const void* a, int dtype, const void* w_in, const float* b_in, const void* w_out,
@@ -513,7 +518,7 @@ int tj_expert_ffn(const void* a, int dtype, const void* w_in, const float* b_in,
   const int slots = rows * top_k;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   void* h16 = ws;
-  void* y16 = ws + align_up((size_t)slots * ffn_dim * 2, 256);
+  void* y = ws + align_up((size_t)slots * ffn_dim * 2, 256);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   ExpertGemmArgs g{};
   g.a = a;
@@ -530,7 +535,7 @@ int tj_expert_ffn(const void* a, int dtype, const void* w_in, const float* b_in,
   g.N = ffn_dim;
   g.K = d_model;
   g.out = h16;
-  g.workspace = y16;
+  g.workspace = y;
   g.workspace_bytes = (int64_t)slots * d_model * 2;
   rc = launch_experts_gemm(g, s);
   if (rc) return rc;
@@ -539,14 +544,16 @@ int tj_expert_ffn(const void* a, int dtype, const void* w_in, const float* b_in,
   g.bias = b_out;
   g.gather = 0;
   g.gelu = 0;
+  g.out_f32 = 1;
   g.a_rows = slots;
   g.N = d_model;
   g.K = ffn_dim;
-  g.out = y16;
+  g.out = y;
   rc = launch_experts_gemm(g, s);
   if (rc) return rc;
-  return finish(launch_expert_combine(dtype, y16, weights, plan_row_slot(plan, num_experts, rows, top_k), row_count,
-                                      rows, top_k, d_model, out, s),
+  return finish(launch_expert_combine(dtype, experts_gemm_splits(slots, num_experts, d_model, ffn_dim), y, weights,
+                                      plan_row_slot(plan, num_experts, rows, top_k), row_count, rows, top_k, d_model,
+                                      out, s),
                 s);
 }
 

@@ -24,6 +24,11 @@
 // proxy fence (about 1800 cycles with copies in flight) per stage.  48002
 // slots, D 1024, F 4096: 1590 us by TMA gathers, 620 us by cp.async, 310 us
 // from a permuted copy, which expert_gather_kernel writes in about 30 us.
+// The FFN-out of tj_expert_ffn leaves fp32 (expert_combine sums it), straight
+// from the registers: 32 lanes are 32 features, whole 128-byte lines.  With few
+// tiles its K is cut into `splits` parts, each its own tile with its own plane
+// of the output, which the combine adds up: no CTA waits for another, and one
+// token's two experts keep every SM loading weights.
 // Two accumulators overlap a tile's epilogue with the next tile's products.
 // Every CTA reads the plan's offsets and derives the tile list itself: the
 // host never learns the counts.
@@ -59,6 +64,7 @@ struct XpParams {
   const float* bias;        // [E][N] or null
   void* out;                // [slots][N]
   int slots, rows, E, N, K;
+  int splits;               // parts of K; part i writes plane i of out [splits][slots][N]
 };
 
 __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, uint32_t cluster_bar, int c0,
@@ -95,9 +101,9 @@ struct XpType<__nv_bfloat16> {
   static constexpr uint32_t kFormat = (1u << 7) | (1u << 10);
 };
 
-// One tile: `n` tokens from slot s0, features [m0, m0+128) of expert e.
+// One tile: `n` tokens from slot s0, features from m0 of expert e, part `split` of K.
 struct XpTile {
-  int e, s0, n, m0;
+  int e, s0, n, m0, split;
 };
 
 // Walks the tiles of all experts in order.  first[e]: first slot of expert e;
@@ -107,17 +113,22 @@ template <int BN, int kStep, int kFeatures>
 struct XpWalk {
   const int* first;
   const int* tiles;
-  int m_tiles;
+  int m_tiles, splits;
   int e = 0;
-  __device__ XpWalk(const int* f, const int* t, int m) : first(f), tiles(t), m_tiles(m) {}
+  __device__ XpWalk(const int* f, const int* t, int m, int s) : first(f), tiles(t), m_tiles(m), splits(s) {}
   __device__ XpTile at(int t) {
     while (t >= tiles[e + 1]) ++e;
     const int n = first[e + 1] - first[e];
     const int cuts = (n + BN - 1) / BN;
     const int size = ((n + cuts - 1) / cuts + kStep - 1) / kStep * kStep;
-    const int local = t - tiles[e];
-    const int cut = local / m_tiles;
+    int local = t - tiles[e];
     XpTile r;
+    r.split = 0;
+    if (splits > 1) {
+      r.split = local % splits;
+      local /= splits;
+    }
+    const int cut = local / m_tiles;
     r.e = e;
     r.s0 = first[e] + cut * size;
     r.n = min(size, first[e + 1] - r.s0);
@@ -126,7 +137,8 @@ struct XpWalk {
   }
 };
 
-template <bool kPair, int BN, bool kGelu, bool kGather, typename T>
+// Out: T, or float for the fp32 planes.
+template <bool kPair, int BN, bool kGelu, bool kGather, typename T, typename Out>
 __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const CUtensorMap& tmX, const XpParams& p) {
   using Cfg = XpCfg<kPair, BN>;
   using Walk = XpWalk<BN, Cfg::kStep, Cfg::kFeatures>;
@@ -190,7 +202,7 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
   for (int e = threadIdx.x; e < p.E; e += kXpThreads) {
     const int n = first[e + 1] - first[e];
     if (n < 0) report_error(kDevBadArgument, 244);
-    tiles[e] = n > 0 ? (n + BN - 1) / BN * m_tiles : 0;
+    tiles[e] = n > 0 ? (n + BN - 1) / BN * m_tiles * p.splits : 0;
   }
   __syncthreads();
   if (warp == 0) {
@@ -204,19 +216,20 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
   const uint32_t tmem_base = *tmem_slot;
   const int total_tiles = tiles[p.E];
   const int k_blocks = (p.K + kBK - 1) / kBK;
+  const int k_part = (k_blocks + p.splits - 1) / p.splits;  // the host leaves no part empty
   const int tile0 = (int)blockIdx.x / kCtas;
   const int tile_step = (int)gridDim.x / kCtas;
 
   if (warp == 0) {
     if (lane == 0) {
-      Walk walk(first, tiles, m_tiles);
+      Walk walk(first, tiles, m_tiles, p.splits);
       int stage = 0;
       uint32_t phase = 0;
       int last_parity[S];
       for (int s = 0; s < S; ++s) last_parity[s] = -1;
       for (int t = tile0; t < total_tiles && !*abort_flag; t += tile_step) {
         const XpTile tile = walk.at(t);
-        for (int kb = 0; kb < k_blocks; ++kb) {
+        for (int kb = tile.split * k_part; kb < min(k_blocks, (tile.split + 1) * k_part); ++kb) {
           if (!mbar_wait(empty_bar(stage), phase ^ 1, abort_flag, 250)) break;
           if (leader) mbar_arrive_expect_tx(full_bar(stage), kCtas * Cfg::kWBytes);
           const uint32_t dst = smem_u32(sW + stage * Cfg::kWBytes);
@@ -238,7 +251,7 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
           if (last_parity[s] >= 0) drain_wait(full_bar(s), (uint32_t)last_parity[s]);
     }
   } else if (warp == 1) {
-    Walk walk(first, tiles, m_tiles);
+    Walk walk(first, tiles, m_tiles, p.splits);
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
@@ -257,7 +270,7 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
           row[i] = min(max(r, 0), p.rows - 1);
         }
       }
-      for (int kb = 0; kb < k_blocks; ++kb) {
+      for (int kb = tile.split * k_part; kb < min(k_blocks, (tile.split + 1) * k_part); ++kb) {
         ok = mbar_wait(empty_bar(stage), phase ^ 1, abort_flag, 251);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
@@ -280,7 +293,7 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
     }
   } else if (warp == 2) {
     if (leader && lane == 0) {
-      Walk walk(first, tiles, m_tiles);
+      Walk walk(first, tiles, m_tiles, p.splits);
       int stage = 0;
       uint32_t phase = 0;
       int acc = 0;
@@ -294,7 +307,7 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
         bool ok = true;
-        for (int kb = 0; kb < k_blocks; ++kb) {
+        for (int kb = tile.split * k_part; kb < min(k_blocks, (tile.split + 1) * k_part); ++kb) {
           if (!mbar_wait<kPair>(full_bar(stage), phase, abort_flag, 253)) {
             ok = false;
             break;
@@ -306,9 +319,9 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
           for (int k = 0; k < kBK / 16; ++k) {
             const uint64_t ak = a_desc + (uint64_t)(2 * k), bk = b_desc + (uint64_t)(2 * k);
             if constexpr (kPair)
-              mma_f16_ss_pair(d_tmem, ak, bk, idesc, (kb | k) != 0 ? 1u : 0u);
+              mma_f16_ss_pair(d_tmem, ak, bk, idesc, kb != tile.split * k_part || k != 0 ? 1u : 0u);
             else
-              mma_f16_ss(d_tmem, ak, bk, idesc, (kb | k) != 0 ? 1u : 0u);
+              mma_f16_ss(d_tmem, ak, bk, idesc, kb != tile.split * k_part || k != 0 ? 1u : 0u);
           }
           issued = true;
           if constexpr (kPair) {
@@ -343,7 +356,7 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
       }
     }
   } else if (warp >= 4) {
-    Walk walk(first, tiles, m_tiles);
+    Walk walk(first, tiles, m_tiles, p.splits);
     const int quarter = warp & 3;
     const int group = (warp - 4) >> 2;
     const int tid = quarter * 32 + lane;  // feature inside this CTA's 128
@@ -354,7 +367,7 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
     for (int t = tile0; t < total_tiles; t += tile_step) {
       XpTile tile = walk.at(t);
       tile.m0 += rank * kBM;
-      const float bias = (p.bias && tile.m0 + tid < p.N) ? __ldg(p.bias + (int64_t)tile.e * p.N + tile.m0 + tid) : 0.f;
+      const float bias = (p.bias && tile.split == 0 && tile.m0 + tid < p.N) ? __ldg(p.bias + (int64_t)tile.e * p.N + tile.m0 + tid) : 0.f;
       const bool ok = mbar_wait(tfull_bar(acc), acc_phase, abort_flag, 254);
       // The four warps of a group meet at barriers below, so they leave together.
       if (named_barrier_any(bar_id, 128, !ok)) break;
@@ -364,6 +377,15 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
         uint32_t r[32];
         tmem_ld32(t_row + (uint32_t)c, r);
         tmem_ld_wait();
+        if constexpr (sizeof(Out) == 4) {
+          float* o = static_cast<float*>(p.out) + ((int64_t)tile.split * p.slots + tile.s0 + c) * p.N + tile.m0 + tid;
+          if (tile.m0 + tid < p.N) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c + i < tile.n) o[(int64_t)i * p.N] = __uint_as_float(r[i]) + bias;
+          }
+          continue;
+        }
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           float2 v = make_float2(__uint_as_float(r[2 * i]) + bias, __uint_as_float(r[2 * i + 1]) + bias);
@@ -414,22 +436,22 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
   }
 }
 
-template <int BN, bool kGelu, bool kGather, typename T>
+template <int BN, bool kGelu, bool kGather, typename T, typename Out>
 __global__ void __launch_bounds__(kXpThreads, 1)
     experts_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                         const XpParams p) {
-  experts_gemm_body<false, BN, kGelu, kGather, T>(tmW, tmX, p);
+  experts_gemm_body<false, BN, kGelu, kGather, T, Out>(tmW, tmX, p);
 }
 
-template <int BN, bool kGelu, typename T>
+template <int BN, bool kGelu, typename T, typename Out>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kXpThreads, 1)
     experts_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                              const XpParams p) {
-  experts_gemm_body<true, BN, kGelu, false, T>(tmW, tmX, p);
+  experts_gemm_body<true, BN, kGelu, false, T, Out>(tmW, tmX, p);
 }
 
 // CTAs to launch at most: one per SM, for pairs as many as fit in clusters.
-template <bool kPair, int BN, bool kGelu, bool kGather, typename T>
+template <bool kPair, int BN, bool kGelu, bool kGather, typename T, typename Out>
 static int experts_gemm_ctas(int* ctas) {
   using Cfg = XpCfg<kPair, BN>;
   int num_sms = 0;
@@ -440,9 +462,9 @@ static int experts_gemm_ctas(int* ctas) {
   if (cached == 0) {
     void (*kernel)(CUtensorMap, CUtensorMap, XpParams);
     if constexpr (kPair)
-      kernel = experts_gemm_pair_kernel<BN, kGelu, T>;
+      kernel = experts_gemm_pair_kernel<BN, kGelu, T, Out>;
     else
-      kernel = experts_gemm_kernel<BN, kGelu, kGather, T>;
+      kernel = experts_gemm_kernel<BN, kGelu, kGather, T, Out>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)Cfg::smem_bytes(kRouteMaxExperts));
     if (e != cudaSuccess) return set_error(TJ_ERR_CUDA, "gemm_experts smem attribute: %s", cudaGetErrorString(e));
@@ -463,7 +485,7 @@ static int experts_gemm_ctas(int* ctas) {
   return TJ_OK;
 }
 
-template <bool kPair, int BN, bool kGelu, bool kGather, typename T>
+template <bool kPair, int BN, bool kGelu, bool kGather, typename T, typename Out>
 static int launch_experts_gemm_t(const ExpertGemmArgs& a, const XpParams& kp, cudaStream_t stream) {
   using Cfg = XpCfg<kPair, BN>;
   CUtensorMap tw, tx;
@@ -478,20 +500,20 @@ static int launch_experts_gemm_t(const ExpertGemmArgs& a, const XpParams& kp, cu
   rc = make_tmap_f16(&tx, a.a, 2, dx, sx, bx);
   if (rc) return rc;
   int ctas = 0;
-  rc = experts_gemm_ctas<kPair, BN, kGelu, kGather, T>(&ctas);
+  rc = experts_gemm_ctas<kPair, BN, kGelu, kGather, T, Out>(&ctas);
   if (rc) return rc;
   const int64_t m_tiles = (a.N + Cfg::kFeatures - 1) / Cfg::kFeatures;
   const int64_t reached = a.slots < a.num_experts ? a.slots : a.num_experts;
-  const int64_t max_tiles = (a.slots / BN + reached) * m_tiles;
+  const int64_t max_tiles = (a.slots / BN + reached) * m_tiles * kp.splits;
   if (max_tiles > INT32_MAX) return set_error(TJ_ERR_UNSUPPORTED, "gemm_experts: too many tiles");
   const int64_t want = max_tiles * (kPair ? 2 : 1);
   const int grid = (int)(want < ctas ? want : ctas);
   cudaError_t e;
   if constexpr (kPair)
-    e = launch_pdl(experts_gemm_pair_kernel<BN, kGelu, T>, dim3(grid), dim3(kXpThreads),
+    e = launch_pdl(experts_gemm_pair_kernel<BN, kGelu, T, Out>, dim3(grid), dim3(kXpThreads),
                    Cfg::smem_bytes(a.num_experts), stream, tw, tx, kp);
   else
-    e = launch_pdl(experts_gemm_kernel<BN, kGelu, kGather, T>, dim3(grid), dim3(kXpThreads),
+    e = launch_pdl(experts_gemm_kernel<BN, kGelu, kGather, T, Out>, dim3(grid), dim3(kXpThreads),
                    Cfg::smem_bytes(a.num_experts), stream, tw, tx, kp);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(TJ_ERR_CUDA, "gemm_experts launch: %s", cudaGetErrorString(e));
@@ -501,11 +523,15 @@ static int launch_experts_gemm_t(const ExpertGemmArgs& a, const XpParams& kp, cu
 template <bool kPair, int BN, bool kGather>
 static int launch_experts_gemm_bn(const ExpertGemmArgs& a, const XpParams& kp, cudaStream_t stream) {
   const bool bf16 = a.dtype == TJ_DTYPE_BF16;
+  if constexpr (!kGather)
+    if (a.out_f32)
+      return bf16 ? launch_experts_gemm_t<kPair, BN, false, false, __nv_bfloat16, float>(a, kp, stream)
+                  : launch_experts_gemm_t<kPair, BN, false, false, __half, float>(a, kp, stream);
   if (a.gelu)
-    return bf16 ? launch_experts_gemm_t<kPair, BN, true, kGather, __nv_bfloat16>(a, kp, stream)
-                : launch_experts_gemm_t<kPair, BN, true, kGather, __half>(a, kp, stream);
-  return bf16 ? launch_experts_gemm_t<kPair, BN, false, kGather, __nv_bfloat16>(a, kp, stream)
-              : launch_experts_gemm_t<kPair, BN, false, kGather, __half>(a, kp, stream);
+    return bf16 ? launch_experts_gemm_t<kPair, BN, true, kGather, __nv_bfloat16, __nv_bfloat16>(a, kp, stream)
+                : launch_experts_gemm_t<kPair, BN, true, kGather, __half, __half>(a, kp, stream);
+  return bf16 ? launch_experts_gemm_t<kPair, BN, false, kGather, __nv_bfloat16, __nv_bfloat16>(a, kp, stream)
+              : launch_experts_gemm_t<kPair, BN, false, kGather, __half, __half>(a, kp, stream);
 }
 
 // Permuted copy: out[s] = a[slot_row[s]] for the plan's slots, 16 bytes a
@@ -558,6 +584,19 @@ static int launch_expert_gather(const ExpertGemmArgs& a, void* out, cudaStream_t
 // 32 on average, else one CTA with tiles of up to 32.
 static bool experts_gemm_pairs(int64_t slots, int num_experts) { return slots > 32 * (int64_t)num_experts; }
 
+// Parts of K for the fp32 planes: while the experts have few rows and the
+// tiles (each of the experts that can be reached, 128 features) do not give
+// every SM about four, and a part keeps four K steps of 64.
+int experts_gemm_splits(int64_t slots, int num_experts, int n, int k) {
+  if (experts_gemm_pairs(slots, num_experts)) return 1;
+  const int64_t tiles = (slots < num_experts ? slots : num_experts) * ((n + kBM - 1) / kBM);
+  const int k_blocks = (k + kBK - 1) / kBK;
+  int splits = 1;
+  while (2 * splits * 4 <= k_blocks && tiles * splits < 4 * 148) splits *= 2;
+  const int part = (k_blocks + splits - 1) / splits;
+  return (k_blocks + part - 1) / part;  // none of them empty
+}
+
 int64_t experts_gemm_workspace(int64_t slots, int num_experts, int k, int gather) {
   return gather && experts_gemm_pairs(slots, num_experts) ? slots * k * 2 : 0;
 }
@@ -589,6 +628,7 @@ int launch_experts_gemm(const ExpertGemmArgs& a, cudaStream_t stream) {
   kp.E = a.num_experts;
   kp.N = a.N;
   kp.K = a.K;
+  kp.splits = a.out_f32 ? experts_gemm_splits(a.slots, a.num_experts, a.N, a.K) : 1;
   if (experts_gemm_pairs(a.slots, a.num_experts)) {
     ExpertGemmArgs g = a;
     if (a.gather) {

@@ -163,15 +163,18 @@ struct ExpertGemmArgs {
   const int32_t* offsets;   // [num_experts+1]
   const int32_t* slot_row;  // [slots]
   int dtype, gather, gelu;
+  int out_f32;              // out: float [experts_gemm_splits][slots][N] (not with gather or gelu)
   int slots, a_rows, num_experts, N, K;
   void* out;                // [slots][N]
   void* workspace;          // gather: experts_gemm_workspace bytes
   int64_t workspace_bytes;
 };
+int experts_gemm_splits(int64_t slots, int num_experts, int n, int k);
 int64_t experts_gemm_workspace(int64_t slots, int num_experts, int k, int gather);
 int launch_experts_gemm(const ExpertGemmArgs& args, cudaStream_t stream);
 
-int launch_expert_combine(int dtype, const void* y, const float* weights, const int32_t* row_slot,
+// y: dtype [slots][D], or with planes > 0 float [planes][slots][D].
+int launch_expert_combine(int dtype, int planes, const void* y, const float* weights, const int32_t* row_slot,
                           const int32_t* row_count, int rows, int top_k, int D, void* out, cudaStream_t stream);
 
 int launch_sandwich_norm(const tj_sandwich_desc& desc, cudaStream_t stream);

@@ -339,9 +339,11 @@ int launch_sandwich_norm(const tj_sandwich_desc& d, cudaStream_t stream) {
 }
 
 // out[t] = sum_j weights[t,j] * y[row_slot[t,j]] (fp32 sum, one rounding);
-// zeros for a row without an expert.  One thread per 8 columns.
-template <typename T>
-__global__ void __launch_bounds__(256) expert_combine_kernel(const T* __restrict__ y, const float* __restrict__ weights,
+// zeros for a row without an expert.  y is T [slots][D], or fp32 planes
+// [planes][slots][D] whose sum is the expert's output.  One thread per 8 columns.
+template <typename T, typename Y>
+__global__ void __launch_bounds__(256) expert_combine_kernel(const Y* __restrict__ y, int planes,
+                                                             const float* __restrict__ weights,
                                                              const int32_t* __restrict__ row_slot,
                                                              const int32_t* __restrict__ row_count, int rows,
                                                              int top_k, int D, int64_t slots, T* __restrict__ out) {
@@ -364,14 +366,32 @@ __global__ void __launch_bounds__(256) expert_combine_kernel(const T* __restrict
       continue;
     }
     float v[8];
-    row_load_16<8, T>(y + (int64_t)slot * D, g, v);
+    if constexpr (sizeof(Y) == 4) {
+      row_load_f32<8>(y + (int64_t)slot * D, g, v);
+      for (int q = 1; q < planes; ++q) {
+        float u[8];
+        row_load_f32<8>(y + ((int64_t)q * slots + slot) * D, g, u);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += u[e];
+      }
+    } else {
+      row_load_16<8, T>(y + (int64_t)slot * D, g, v);
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] = fmaf(w, v[e], acc[e]);
   }
   row_store_16<8, T>(out + row * D, g, acc);
 }
 
-int launch_expert_combine(int dtype, const void* y, const float* weights, const int32_t* row_slot,
+template <typename T, typename Y>
+static cudaError_t launch_combine_t(int planes, const void* y, const float* weights, const int32_t* row_slot,
+                                    const int32_t* row_count, int rows, int top_k, int D, void* out, unsigned blocks,
+                                    cudaStream_t stream) {
+  return launch_pdl(expert_combine_kernel<T, Y>, dim3(blocks), dim3(256), 0, stream, static_cast<const Y*>(y), planes,
+                    weights, row_slot, row_count, rows, top_k, D, (int64_t)rows * top_k, static_cast<T*>(out));
+}
+
+int launch_expert_combine(int dtype, int planes, const void* y, const float* weights, const int32_t* row_slot,
                           const int32_t* row_count, int rows, int top_k, int D, void* out, cudaStream_t stream) {
   if (rows < 0 || top_k < 1 || D <= 0 || D % 8 != 0)
     return set_error(TJ_ERR_INVALID_ARGUMENT, "expert_combine: rows=%d top_k=%d d_model=%d (a multiple of 8)", rows,
@@ -388,16 +408,14 @@ int launch_expert_combine(int dtype, const void* y, const float* weights, const 
   const int64_t items = (int64_t)rows * (D / 8);
   const int64_t blocks = (items + 255) / 256;
   if (blocks > INT32_MAX) return set_error(TJ_ERR_UNSUPPORTED, "expert_combine: rows * d_model too large");
-  const int64_t slots = (int64_t)rows * top_k;
+  const unsigned b = (unsigned)blocks;
   cudaError_t e;
   if (dtype == TJ_DTYPE_F16)
-    e = launch_pdl(expert_combine_kernel<__half>, dim3((unsigned)blocks), dim3(256), 0, stream,
-                   static_cast<const __half*>(y), weights, row_slot, row_count, rows, top_k, D, slots,
-                   static_cast<__half*>(out));
+    e = planes ? launch_combine_t<__half, float>(planes, y, weights, row_slot, row_count, rows, top_k, D, out, b, stream)
+               : launch_combine_t<__half, __half>(0, y, weights, row_slot, row_count, rows, top_k, D, out, b, stream);
   else
-    e = launch_pdl(expert_combine_kernel<__nv_bfloat16>, dim3((unsigned)blocks), dim3(256), 0, stream,
-                   static_cast<const __nv_bfloat16*>(y), weights, row_slot, row_count, rows, top_k, D, slots,
-                   static_cast<__nv_bfloat16*>(out));
+    e = planes ? launch_combine_t<__nv_bfloat16, float>(planes, y, weights, row_slot, row_count, rows, top_k, D, out, b, stream)
+               : launch_combine_t<__nv_bfloat16, __nv_bfloat16>(0, y, weights, row_slot, row_count, rows, top_k, D, out, b, stream);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(TJ_ERR_CUDA, "expert_combine launch: %s", cudaGetErrorString(e));
   return TJ_OK;

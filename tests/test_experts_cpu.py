@@ -47,7 +47,7 @@ def test_plan_and_workspace_sizes(pkg):
     assert lib.tj_expert_plan_ints(33, 2, 8) == 9 + 132 + 16
     assert lib.tj_expert_plan_ints(100000, 4, 64) == 65 + 800000 + 148 * 64
     assert lib.tj_expert_plan_ints(-1, 2, 8) == 0 and lib.tj_expert_plan_ints(1, 0, 8) == 0
-    assert lib.tj_expert_ffn_workspace_bytes(10, 2, 4, 64, 128) == 20 * 256 + 20 * 128
+    assert lib.tj_expert_ffn_workspace_bytes(10, 2, 4, 64, 128) == 20 * 256 + 20 * 256
     assert lib.tj_expert_ffn_workspace_bytes(10, 0, 4, 64, 128) == 0
     assert lib.tj_gemm_experts_workspace_bytes(64, 2, 4, 64, 1) == 0  # 32 rows per expert: gathered by the kernel
     assert lib.tj_gemm_experts_workspace_bytes(65, 2, 4, 64, 1) == 130 * 128
