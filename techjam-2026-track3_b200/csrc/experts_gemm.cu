@@ -14,8 +14,10 @@
 //   warp 1       token tiles [tokens x 64] by TMA: consecutive slots, or the
 //                rows of the slots' tokens (TMA row gather, 4 rows per instruction)
 //   warp 2       TMEM allocation and tcgen05.mma (K=16 per instruction)
-//   warps 4-11   epilogue: TMEM -> bias, GELU -> 16 bits -> shared memory
-//                transposed to [token][feature] -> 256-byte rows of `out`
+//   warps 4-11   epilogue: TMEM -> bias, GELU -> 16 bits -> transposed into the
+//                warp's scratch ([token][32 features], stmatrix) -> one bulk
+//                tensor store per 32 tokens; a tile's last, partial 32 tokens by
+//                plain stores, so that the next expert's rows stay as they are
 // With many tokens per expert two CTAs form a pair (tcgen05 cta_group::2): 256
 // features x up to 256 tokens, each CTA loading half of either operand, 32 KB
 // per K step of 64 instead of 48 KB; both CTAs' loads arrive on the leader's
@@ -24,8 +26,7 @@
 // proxy fence (about 1800 cycles with copies in flight) per stage.  48002
 // slots, D 1024, F 4096: 1590 us by TMA gathers, 620 us by cp.async, 310 us
 // from a permuted copy, which expert_gather_kernel writes in about 30 us.
-// The FFN-out of tj_expert_ffn leaves fp32 (expert_combine sums it), straight
-// from the registers: 32 lanes are 32 features, whole 128-byte lines.  With few
+// The FFN-out of tj_expert_ffn leaves fp32 (expert_combine sums it).  With few
 // tiles its K is cut into `splits` parts, each its own tile with its own plane
 // of the output, which the combine adds up: no CTA waits for another, and one
 // token's two experts keep every SM loading weights.
@@ -39,7 +40,9 @@ namespace tj {
 
 constexpr int kXpThreads = 384;
 constexpr int kXpEpiWarps = 8;
-constexpr uint32_t kXpScratchBytes = 2 * 32 * 256;  // per epilogue group: 32 tokens x 128 features
+constexpr int kXpParts = 4;  // of a tile of 256 tokens in a partial last wave
+constexpr uint32_t kXpWarpScratch = 2048;  // per epilogue warp: 32 tokens x 32 features in 16 bits, 16 in fp32
+constexpr uint32_t kXpScratchBytes = kXpEpiWarps * kXpWarpScratch;
 
 // BN: tokens of a tile; with kPair half of them in each CTA.
 template <bool kPair, int BN>
@@ -85,8 +88,27 @@ __device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
-__device__ __forceinline__ void st_shared_u16(uint32_t addr, uint32_t v) {
-  asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"((unsigned short)v) : "memory");
+// 16 lanes x 32 consecutive columns: thread t receives lane t/4 (r[4g], r[4g+1])
+// and t/4 + 8 (r[4g+2], r[4g+3]) of columns 8g + 2(t%4) and the next.
+__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
+__device__ __forceinline__ void st_shared_f32(uint32_t addr, float v) {
+  asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+
+// Four transposed 8x8 blocks of 16-bit values; lane l gives the address of row
+// l%8 of block l/8.
+__device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b),
+               "r"(c), "r"(d)
+               : "memory");
 }
 
 // Operand formats of the instruction descriptor (bits 7-9 and 10-12).
@@ -108,15 +130,36 @@ struct XpTile {
 
 // Walks the tiles of all experts in order.  first[e]: first slot of expert e;
 // tiles[e]: first tile of expert e (tiles[E] = total).  An expert's tokens are
-// cut into equal tiles of a multiple of kStep tokens, at most BN.
-template <int BN, int kStep, int kFeatures>
+// cut into equal tiles of a multiple of kStep tokens, at most BN.  The tiles
+// are dealt out in waves of `step`; if a last, partial wave fills at most half
+// of them its tiles are cut further, into kParts parts at most by tokens (a
+// part may be empty: n <= 0).  48002 slots, D 4096 -> 1024: 10.3 waves, and the
+// last one takes a third of the time.
+template <int BN, int kStep, int kFeatures, int kParts>
 struct XpWalk {
   const int* first;
   const int* tiles;
   int m_tiles, splits;
+  int whole, parts;  // tiles before the last wave, parts of each tile of it
+  int total;         // tiles and parts
   int e = 0;
-  __device__ XpWalk(const int* f, const int* t, int m, int s) : first(f), tiles(t), m_tiles(m), splits(s) {}
+  __device__ XpWalk(const int* f, const int* t, int experts, int m, int s, int step)
+      : first(f), tiles(t), m_tiles(m), splits(s) {
+    const int all = tiles[experts];
+    whole = all;
+    parts = 1;
+    if (kParts > 1 && all % step != 0) {
+      whole = all - all % step;
+      parts = min(kParts, step / (all - whole));
+    }
+    total = whole + (all - whole) * parts;
+  }
   __device__ XpTile at(int t) {
+    int part = 0;
+    if (kParts > 1 && t >= whole) {
+      part = (t - whole) % parts;
+      t = whole + (t - whole) / parts;
+    }
     while (t >= tiles[e + 1]) ++e;
     const int n = first[e + 1] - first[e];
     const int cuts = (n + BN - 1) / BN;
@@ -133,15 +176,21 @@ struct XpWalk {
     r.s0 = first[e] + cut * size;
     r.n = min(size, first[e + 1] - r.s0);
     r.m0 = (local - cut * m_tiles) * kFeatures;
+    if (kParts > 1 && t >= whole && parts > 1) {
+      const int per = ((r.n + parts - 1) / parts + kStep - 1) / kStep * kStep;
+      r.s0 += part * per;
+      r.n = min(per, r.n - part * per);
+    }
     return r;
   }
 };
 
 // Out: T, or float for the fp32 planes.
 template <bool kPair, int BN, bool kGelu, bool kGather, typename T, typename Out>
-__device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const CUtensorMap& tmX, const XpParams& p) {
+__device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const CUtensorMap& tmX,
+                                                  const CUtensorMap& tmO, const XpParams& p) {
   using Cfg = XpCfg<kPair, BN>;
-  using Walk = XpWalk<BN, Cfg::kStep, Cfg::kFeatures>;
+  using Walk = XpWalk<BN, Cfg::kStep, Cfg::kFeatures, kPair ? kXpParts : 1>;
   constexpr int S = Cfg::kStages;
   constexpr int kCtas = kPair ? 2 : 1;
   extern __shared__ uint8_t smem_raw[];
@@ -180,6 +229,7 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
     fence_barrier_init();
     tma_prefetch_desc(&tmW);
     tma_prefetch_desc(&tmX);
+    tma_prefetch_desc(&tmO);
   }
   if (warp == 2) {
     if constexpr (kPair) {
@@ -214,7 +264,6 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
   if constexpr (kPair) cluster_sync();  // the peer's barriers are initialised
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const int total_tiles = tiles[p.E];
   const int k_blocks = (p.K + kBK - 1) / kBK;
   const int k_part = (k_blocks + p.splits - 1) / p.splits;  // the host leaves no part empty
   const int tile0 = (int)blockIdx.x / kCtas;
@@ -222,13 +271,14 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
 
   if (warp == 0) {
     if (lane == 0) {
-      Walk walk(first, tiles, m_tiles, p.splits);
+      Walk walk(first, tiles, p.E, m_tiles, p.splits, tile_step);
       int stage = 0;
       uint32_t phase = 0;
       int last_parity[S];
       for (int s = 0; s < S; ++s) last_parity[s] = -1;
-      for (int t = tile0; t < total_tiles && !*abort_flag; t += tile_step) {
+      for (int t = tile0; t < walk.total && !*abort_flag; t += tile_step) {
         const XpTile tile = walk.at(t);
+        if (tile.n <= 0) continue;
         for (int kb = tile.split * k_part; kb < min(k_blocks, (tile.split + 1) * k_part); ++kb) {
           if (!mbar_wait(empty_bar(stage), phase ^ 1, abort_flag, 250)) break;
           if (leader) mbar_arrive_expect_tx(full_bar(stage), kCtas * Cfg::kWBytes);
@@ -251,12 +301,13 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
           if (last_parity[s] >= 0) drain_wait(full_bar(s), (uint32_t)last_parity[s]);
     }
   } else if (warp == 1) {
-    Walk walk(first, tiles, m_tiles, p.splits);
+    Walk walk(first, tiles, p.E, m_tiles, p.splits, tile_step);
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int t = tile0; t < total_tiles && ok; t += tile_step) {
+    for (int t = tile0; t < walk.total && ok; t += tile_step) {
       const XpTile tile = walk.at(t);
+      if (tile.n <= 0) continue;
       const int cols = (tile.n + Cfg::kStep - 1) / Cfg::kStep * Cfg::kStep / kCtas;  // this CTA's
       constexpr int kRows = kGather ? 4 : Cfg::kBoxRows;                             // of one load
       const int loads = (cols + kRows - 1) / kRows;
@@ -293,14 +344,15 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
     }
   } else if (warp == 2) {
     if (leader && lane == 0) {
-      Walk walk(first, tiles, m_tiles, p.splits);
+      Walk walk(first, tiles, p.E, m_tiles, p.splits, tile_step);
       int stage = 0;
       uint32_t phase = 0;
       int acc = 0;
       uint32_t acc_phase = 0;
       bool issued = false;
-      for (int t = tile0; t < total_tiles && !*abort_flag; t += tile_step) {
+      for (int t = tile0; t < walk.total && !*abort_flag; t += tile_step) {
         const XpTile tile = walk.at(t);
+        if (tile.n <= 0) continue;
         const int cols = (tile.n + Cfg::kStep - 1) / Cfg::kStep * Cfg::kStep;
         const uint32_t idesc = idesc_f16_f32(Cfg::kFeatures, cols, 0, 0) | XpType<T>::kFormat;
         if (!mbar_wait<kPair>(tempty_bar(acc), acc_phase ^ 1, abort_flag, 252)) break;
@@ -356,54 +408,103 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
       }
     }
   } else if (warp >= 4) {
-    Walk walk(first, tiles, m_tiles, p.splits);
+    Walk walk(first, tiles, p.E, m_tiles, p.splits, tile_step);
     const int quarter = warp & 3;
     const int group = (warp - 4) >> 2;
-    const int tid = quarter * 32 + lane;  // feature inside this CTA's 128
-    const uint32_t buf = scratch + (uint32_t)group * (kXpScratchBytes / 2);
-    const int bar_id = 1 + group;
+    const uint32_t buf = scratch + (uint32_t)(warp - 4) * kXpWarpScratch;
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int t = tile0; t < total_tiles; t += tile_step) {
-      XpTile tile = walk.at(t);
-      tile.m0 += rank * kBM;
-      const float bias = (p.bias && tile.split == 0 && tile.m0 + tid < p.N) ? __ldg(p.bias + (int64_t)tile.e * p.N + tile.m0 + tid) : 0.f;
-      const bool ok = mbar_wait(tfull_bar(acc), acc_phase, abort_flag, 254);
-      // The four warps of a group meet at barriers below, so they leave together.
-      if (named_barrier_any(bar_id, 128, !ok)) break;
+    for (int t = tile0; t < walk.total; t += tile_step) {
+      const XpTile tile = walk.at(t);
+      if (tile.n <= 0) continue;
+      const int f0 = tile.m0 + rank * kBM + quarter * 32;  // this warp's 32 features
+      if (!mbar_wait(tfull_bar(acc), acc_phase, abort_flag, 254)) break;
       tc_fence_after();
       const uint32_t t_row = tmem_base + (uint32_t)(acc * BN) + ((uint32_t)(quarter * 32) << 16);
-      for (int c = group * 32; c < tile.n; c += 64) {
-        uint32_t r[32];
-        tmem_ld32(t_row + (uint32_t)c, r);
-        tmem_ld_wait();
-        if constexpr (sizeof(Out) == 4) {
-          float* o = static_cast<float*>(p.out) + ((int64_t)tile.split * p.slots + tile.s0 + c) * p.N + tile.m0 + tid;
-          if (tile.m0 + tid < p.N) {
+      const float* bias = (p.bias && tile.split == 0) ? p.bias + (int64_t)tile.e * p.N : nullptr;
+      if constexpr (sizeof(Out) == 4) {
+        // Thread = feature: a token's 32 values are one 128-byte row.
+        const float b = (bias && f0 + lane < p.N) ? __ldg(bias + f0 + lane) : 0.f;
+        float* plane = static_cast<float*>(p.out) + (int64_t)tile.split * p.slots * p.N;
+        for (int c = group * 32; c < tile.n && f0 < p.N; c += 64) {
+          uint32_t r[32];
+          tmem_ld32(t_row + (uint32_t)c, r);
+          tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (c + i < tile.n) o[(int64_t)i * p.N] = __uint_as_float(r[i]) + bias;
+          for (int h = 0; h < 2; ++h) {  // 16 tokens at a time
+            const int tok = c + 16 * h;
+            if (tok + 16 <= tile.n) {
+              if (lane == 0) bulk_wait_read();  // the last store has read the scratch
+              __syncwarp();
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                st_shared_f32(buf + i * 128 + lane * 4, __uint_as_float(r[16 * h + i]) + b);
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                tma_store_3d(&tmO, buf, f0, tile.s0 + tok, tile.split);
+                bulk_commit();
+              }
+            } else if (f0 + lane < p.N) {
+              float* o = plane + (int64_t)(tile.s0 + tok) * p.N + f0 + lane;
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if (tok + i < tile.n) o[(int64_t)i * p.N] = __uint_as_float(r[16 * h + i]) + b;
+            }
           }
-          continue;
         }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float2 v = make_float2(__uint_as_float(r[2 * i]) + bias, __uint_as_float(r[2 * i + 1]) + bias);
-          if (kGelu) v = gelu2(v);
-          const uint32_t h = pack2<T>(v.x, v.y);
-          st_shared_u16(buf + (2 * i) * 256 + tid * 2, h);
-          st_shared_u16(buf + (2 * i + 1) * 256 + tid * 2, h >> 16);
-        }
-        named_barrier_sync(bar_id, 128);
+      } else {
+        float b[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int q = tid + 128 * i;
-          const int tok = q >> 4, col = tile.m0 + (q & 15) * 8;
-          const uint4 v = ld_shared_v4(buf + (uint32_t)q * 16);
-          if (c + tok < tile.n && col < p.N)
-            *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (int64_t)(tile.s0 + c + tok) * p.N + col) = v;
+          const int f = f0 + 8 * i + (lane >> 2);
+          b[i] = (bias && f < p.N) ? __ldg(bias + f) : 0.f;
         }
-        named_barrier_sync(bar_id, 128);
+        for (int c = group * 32; c < tile.n && f0 < p.N; c += 64) {
+          uint32_t lo[16], hi[16];  // features f0.., f0+16..
+          tmem_ld_16x32(t_row + (uint32_t)c, lo);
+          tmem_ld_16x32(t_row + (16u << 16) + (uint32_t)c, hi);
+          tmem_ld_wait();
+          uint32_t h[4][4];  // [8 tokens][8 features]
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t x = i < 2 ? lo[4 * g + 2 * i] : hi[4 * g + 2 * i - 4];
+              const uint32_t y = i < 2 ? lo[4 * g + 2 * i + 1] : hi[4 * g + 2 * i - 3];
+              float2 v = fadd2(make_float2(__uint_as_float(x), __uint_as_float(y)), make_float2(b[i], b[i]));
+              if (kGelu) v = gelu2(v);
+              h[g][i] = pack2<T>(v.x, v.y);
+            }
+          if (lane == 0) bulk_wait_read();  // the last store has read the scratch
+          __syncwarp();
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const uint32_t row = (uint32_t)(8 * g + (lane & 7));
+            stmatrix_x4_trans(buf + row * 64 + ((((uint32_t)lane >> 3) ^ ((row >> 1) & 3)) << 4), h[g][0], h[g][1],
+                              h[g][2], h[g][3]);
+          }
+          if (c + 32 <= tile.n) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&tmO, buf, f0, tile.s0 + c);
+              bulk_commit();
+            }
+          } else {
+            __syncwarp();
+            const uint32_t piece = (uint32_t)lane & 3;
+            const int col = f0 + 8 * (int)piece;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t row = ((uint32_t)lane >> 2) + 8 * i;
+              const uint4 v = ld_shared_v4(buf + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4));
+              if (c + (int)row < tile.n && col < p.N)
+                *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (int64_t)(tile.s0 + c + (int)row) * p.N + col) = v;
+            }
+            __syncwarp();  // the next chunk rewrites the scratch
+          }
+        }
       }
       tc_fence_before();
       __syncwarp();
@@ -418,6 +519,7 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
         acc_phase ^= 1;
       }
     }
+    if (lane == 0) bulk_wait_all();  // this warp's bulk stores have landed
   }
 
   __syncwarp();
@@ -439,15 +541,15 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
 template <int BN, bool kGelu, bool kGather, typename T, typename Out>
 __global__ void __launch_bounds__(kXpThreads, 1)
     experts_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
-                        const XpParams p) {
-  experts_gemm_body<false, BN, kGelu, kGather, T, Out>(tmW, tmX, p);
+                        const __grid_constant__ CUtensorMap tmO, const XpParams p) {
+  experts_gemm_body<false, BN, kGelu, kGather, T, Out>(tmW, tmX, tmO, p);
 }
 
 template <int BN, bool kGelu, typename T, typename Out>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kXpThreads, 1)
     experts_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
-                             const XpParams p) {
-  experts_gemm_body<true, BN, kGelu, false, T, Out>(tmW, tmX, p);
+                             const __grid_constant__ CUtensorMap tmO, const XpParams p) {
+  experts_gemm_body<true, BN, kGelu, false, T, Out>(tmW, tmX, tmO, p);
 }
 
 // CTAs to launch at most: one per SM, for pairs as many as fit in clusters.
@@ -460,7 +562,7 @@ static int experts_gemm_ctas(int* ctas) {
   static int cache[64] = {};
   int& cached = cache[device_index()];
   if (cached == 0) {
-    void (*kernel)(CUtensorMap, CUtensorMap, XpParams);
+    void (*kernel)(CUtensorMap, CUtensorMap, CUtensorMap, XpParams);
     if constexpr (kPair)
       kernel = experts_gemm_pair_kernel<BN, kGelu, T, Out>;
     else
@@ -488,7 +590,7 @@ static int experts_gemm_ctas(int* ctas) {
 template <bool kPair, int BN, bool kGelu, bool kGather, typename T, typename Out>
 static int launch_experts_gemm_t(const ExpertGemmArgs& a, const XpParams& kp, cudaStream_t stream) {
   using Cfg = XpCfg<kPair, BN>;
-  CUtensorMap tw, tx;
+  CUtensorMap tw, tx, to;
   uint64_t dw[3] = {(uint64_t)a.K, (uint64_t)a.N, (uint64_t)a.num_experts};
   uint64_t sw[2] = {(uint64_t)a.K, (uint64_t)a.K * (uint64_t)a.N};
   uint32_t bw[3] = {kBK, kBM, 1};
@@ -499,6 +601,18 @@ static int launch_experts_gemm_t(const ExpertGemmArgs& a, const XpParams& kp, cu
   uint32_t bx[2] = {kBK, kGather ? 1u : (uint32_t)Cfg::kBoxRows};
   rc = make_tmap_f16(&tx, a.a, 2, dx, sx, bx);
   if (rc) return rc;
+  if constexpr (sizeof(Out) == 4) {
+    uint64_t dn[3] = {(uint64_t)a.N, (uint64_t)a.slots, (uint64_t)kp.splits};
+    uint64_t sn[2] = {(uint64_t)a.N, (uint64_t)a.N * (uint64_t)a.slots};
+    uint32_t bn[3] = {32, 16, 1};
+    rc = make_tmap(&to, a.out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, 3, dn, sn, bn, CU_TENSOR_MAP_SWIZZLE_NONE);
+  } else {
+    uint64_t dn[2] = {(uint64_t)a.N, (uint64_t)a.slots};
+    uint64_t sn[1] = {(uint64_t)a.N};
+    uint32_t bn[2] = {32, 32};
+    rc = make_tmap_f16_sw(&to, a.out, 2, dn, sn, bn, CU_TENSOR_MAP_SWIZZLE_64B);
+  }
+  if (rc) return rc;
   int ctas = 0;
   rc = experts_gemm_ctas<kPair, BN, kGelu, kGather, T, Out>(&ctas);
   if (rc) return rc;
@@ -506,15 +620,15 @@ static int launch_experts_gemm_t(const ExpertGemmArgs& a, const XpParams& kp, cu
   const int64_t reached = a.slots < a.num_experts ? a.slots : a.num_experts;
   const int64_t max_tiles = (a.slots / BN + reached) * m_tiles * kp.splits;
   if (max_tiles > INT32_MAX) return set_error(TJ_ERR_UNSUPPORTED, "gemm_experts: too many tiles");
-  const int64_t want = max_tiles * (kPair ? 2 : 1);
+  const int64_t want = max_tiles * (kPair ? 2 * kXpParts : 1);
   const int grid = (int)(want < ctas ? want : ctas);
   cudaError_t e;
   if constexpr (kPair)
     e = launch_pdl(experts_gemm_pair_kernel<BN, kGelu, T, Out>, dim3(grid), dim3(kXpThreads),
-                   Cfg::smem_bytes(a.num_experts), stream, tw, tx, kp);
+                   Cfg::smem_bytes(a.num_experts), stream, tw, tx, to, kp);
   else
     e = launch_pdl(experts_gemm_kernel<BN, kGelu, kGather, T, Out>, dim3(grid), dim3(kXpThreads),
-                   Cfg::smem_bytes(a.num_experts), stream, tw, tx, kp);
+                   Cfg::smem_bytes(a.num_experts), stream, tw, tx, to, kp);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(TJ_ERR_CUDA, "gemm_experts launch: %s", cudaGetErrorString(e));
   return TJ_OK;
@@ -534,9 +648,10 @@ static int launch_experts_gemm_bn(const ExpertGemmArgs& a, const XpParams& kp, c
               : launch_experts_gemm_t<kPair, BN, false, kGather, __half, __half>(a, kp, stream);
 }
 
-// Permuted copy: out[s] = a[slot_row[s]] for the plan's slots, 16 bytes a
-// thread (rows are whole 16-byte units).  Reads and writes each byte once; what
-// it writes stays in L2 for the products that follow, as far as it fits.
+// Permuted copy: out[s] = a[slot_row[s]] for the plan's slots, a warp per slot,
+// 16 bytes a lane (rows are whole 16-byte units).  Reads and writes each byte
+// once; what it writes stays in L2 for the products that follow, as far as it
+// fits.
 __global__ void __launch_bounds__(256) expert_gather_kernel(const uint4* __restrict__ a,
                                                             const int32_t* __restrict__ offsets,
                                                             const int32_t* __restrict__ slot_row, int slots, int rows,
@@ -544,25 +659,21 @@ __global__ void __launch_bounds__(256) expert_gather_kernel(const uint4* __restr
   pdl_wait();
   pdl_trigger();
   const int used = min(max(offsets[E], 0), slots);
-  const int64_t n = (int64_t)used * units;
-  const int64_t step = (int64_t)gridDim.x * 256;
-  int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  constexpr int kFlight = 4;  // loads in flight per thread
-  for (; i < n; i += kFlight * step) {
-    uint4 v[kFlight];
+  const int lane = threadIdx.x & 31;
+  for (int s = (int)blockIdx.x * 8 + (threadIdx.x >> 5); s < used; s += (int)gridDim.x * 8) {
+    const int r = __ldg(slot_row + s);
+    if ((r < 0 || r >= rows) && lane == 0) report_error(kDevBadArgument, 246);
+    const uint4* from = a + (int64_t)min(max(r, 0), rows - 1) * units;
+    uint4* to = out + (int64_t)s * units;
+    for (int u = lane; u < units; u += 128) {
+      uint4 v[4];
 #pragma unroll
-    for (int u = 0; u < kFlight; ++u) {
-      const int64_t j = i + u * step;
-      if (j < n) {
-        const int s = (int)(j / units);
-        const int r = __ldg(slot_row + s);
-        if (r < 0 || r >= rows) report_error(kDevBadArgument, 246);
-        v[u] = __ldg(a + (int64_t)min(max(r, 0), rows - 1) * units + (j - (int64_t)s * units));
-      }
+      for (int i = 0; i < 4; ++i)
+        if (u + 32 * i < units) v[i] = __ldg(from + u + 32 * i);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (u + 32 * i < units) to[u + 32 * i] = v[i];
     }
-#pragma unroll
-    for (int u = 0; u < kFlight; ++u)
-      if (i + u * step < n) out[i + u * step] = v[u];
   }
 }
 
@@ -571,7 +682,7 @@ static int launch_expert_gather(const ExpertGemmArgs& a, void* out, cudaStream_t
   int num_sms = 0;
   int rc = ensure_device_props(&num_sms);
   if (rc) return rc;
-  const int64_t blocks = ((int64_t)a.slots * units + 1023) / 1024;
+  const int64_t blocks = ((int64_t)a.slots + 7) / 8;
   const int grid = (int)(blocks < 8 * num_sms ? blocks : 8 * num_sms);
   cudaError_t e = launch_pdl(expert_gather_kernel, dim3(grid), dim3(256), 0, stream, static_cast<const uint4*>(a.a),
                              a.offsets, a.slot_row, a.slots, a.a_rows, a.num_experts, units, static_cast<uint4*>(out));

@@ -764,10 +764,12 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-// fp16 tensor map of rank 2..5 with the given swizzle.  dims/strides are in
-// elements, innermost first; strides has rank-1 entries (dims 1..rank-1).
-static int make_tmap_f16_sw(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
-                            const uint64_t* strides_elems, const uint32_t* box, CUtensorMapSwizzle swizzle) {
+// Tensor map of rank 2..5 with the given element type and swizzle.
+// dims/strides are in elements, innermost first; strides has rank-1 entries
+// (dims 1..rank-1).
+static int make_tmap(CUtensorMap* map, const void* base, CUtensorMapDataType type, int elem_bytes, int rank,
+                     const uint64_t* dims, const uint64_t* strides_elems, const uint32_t* box,
+                     CUtensorMapSwizzle swizzle) {
   auto fn = encode_fn();
   if (!fn) return set_error(TJ_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
   cuuint64_t gdim[5];
@@ -779,8 +781,8 @@ static int make_tmap_f16_sw(CUtensorMap* map, const void* base, int rank, const 
     bdim[i] = box[i];
     estride[i] = 1;
   }
-  for (int i = 0; i + 1 < rank; ++i) gstride[i] = strides_elems[i] * 2;
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank, const_cast<void*>(base),
+  for (int i = 0; i + 1 < rank; ++i) gstride[i] = strides_elems[i] * elem_bytes;
+  CUresult r = fn(map, type, (cuuint32_t)rank, const_cast<void*>(base),
                   gdim, gstride, bdim, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -788,6 +790,13 @@ static int make_tmap_f16_sw(CUtensorMap* map, const void* base, int rank, const 
     return set_error(TJ_ERR_INVALID_ARGUMENT, "cuTensorMapEncodeTiled failed (%d) rank=%d", (int)r,
                      rank);
   return TJ_OK;
+}
+
+// 16-bit tensor map of rank 2..5 with the given swizzle (bf16 tiles too: the
+// copies move bits and fill with zeros).
+static int make_tmap_f16_sw(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
+                            const uint64_t* strides_elems, const uint32_t* box, CUtensorMapSwizzle swizzle) {
+  return make_tmap(map, base, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, rank, dims, strides_elems, box, swizzle);
 }
 
 // fp16 tensor map of rank 2..5 with a 128-byte swizzle (the operand tiles).

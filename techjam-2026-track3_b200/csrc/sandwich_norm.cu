@@ -340,7 +340,8 @@ int launch_sandwich_norm(const tj_sandwich_desc& d, cudaStream_t stream) {
 
 // out[t] = sum_j weights[t,j] * y[row_slot[t,j]] (fp32 sum, one rounding);
 // zeros for a row without an expert.  y is T [slots][D], or fp32 planes
-// [planes][slots][D] whose sum is the expert's output.  One thread per 8 columns.
+// [planes][slots][D] whose sum is the expert's output.  A warp per row and 256
+// columns, eight columns a lane.
 template <typename T, typename Y>
 __global__ void __launch_bounds__(256) expert_combine_kernel(const Y* __restrict__ y, int planes,
                                                              const float* __restrict__ weights,
@@ -350,37 +351,43 @@ __global__ void __launch_bounds__(256) expert_combine_kernel(const Y* __restrict
   pdl_wait();
   pdl_trigger();
   const int limit = row_count ? min(rows, *row_count) : rows;
-  const int groups = D / 8;
-  const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = item / groups;
-  const int g = (int)(item - row * groups);
-  if (row >= limit) return;
+  const unsigned segments = ((unsigned)D + 255u) / 256u;
+  const unsigned item = blockIdx.x * 8u + (threadIdx.x >> 5);
+  const int row = (int)(item / segments);
+  const int g = (int)(item - (unsigned)row * segments) * 32 + (int)(threadIdx.x & 31);
+  if (row >= limit || g * 8 >= D) return;
+  const int64_t base = (int64_t)row * top_k;
   float acc[8] = {};
-#pragma unroll 4
+#pragma unroll 2
   for (int j = 0; j < top_k; ++j) {
-    const int slot = __ldg(row_slot + row * top_k + j);
-    const float w = __ldg(weights + row * top_k + j);
+    const int slot = __ldg(row_slot + base + j);
+    const float w = __ldg(weights + base + j);
     if (slot < 0) continue;
     if (slot >= slots) {
       report_error(kDevBadArgument, 243);
       continue;
     }
-    float v[8];
     if constexpr (sizeof(Y) == 4) {
-      row_load_f32<8>(y + (int64_t)slot * D, g, v);
-      for (int q = 1; q < planes; ++q) {
-        float u[8];
-        row_load_f32<8>(y + ((int64_t)q * slots + slot) * D, g, u);
+      for (int q = 0; q < planes; q += 4) {  // up to four planes' loads in flight
+        float v[4][8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += u[e];
+        for (int i = 0; i < 4; ++i)
+          if (q + i < planes) row_load_f32<8>(y + ((int64_t)(q + i) * slots + slot) * D, g, v[i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (q + i < planes) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] = fmaf(w, v[i][e], acc[e]);
+          }
       }
     } else {
+      float v[8];
       row_load_16<8, T>(y + (int64_t)slot * D, g, v);
-    }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = fmaf(w, v[e], acc[e]);
+      for (int e = 0; e < 8; ++e) acc[e] = fmaf(w, v[e], acc[e]);
+    }
   }
-  row_store_16<8, T>(out + row * D, g, acc);
+  row_store_16<8, T>(out + (int64_t)row * D, g, acc);
 }
 
 template <typename T, typename Y>
@@ -405,9 +412,9 @@ int launch_expert_combine(int dtype, int planes, const void* y, const float* wei
       ((reinterpret_cast<uintptr_t>(weights) | reinterpret_cast<uintptr_t>(row_slot) |
         reinterpret_cast<uintptr_t>(row_count)) & 3u))
     return set_error(TJ_ERR_INVALID_ARGUMENT, "expert_combine: misaligned pointer");
-  const int64_t items = (int64_t)rows * (D / 8);
-  const int64_t blocks = (items + 255) / 256;
-  if (blocks > INT32_MAX) return set_error(TJ_ERR_UNSUPPORTED, "expert_combine: rows * d_model too large");
+  const int64_t items = (int64_t)rows * ((D + 255) / 256);
+  if (items > INT32_MAX) return set_error(TJ_ERR_UNSUPPORTED, "expert_combine: rows * d_model too large");
+  const int64_t blocks = (items + 7) / 8;
   const unsigned b = (unsigned)blocks;
   cudaError_t e;
   if (dtype == TJ_DTYPE_F16)
