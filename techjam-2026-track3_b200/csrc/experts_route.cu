@@ -1,6 +1,6 @@
 // Routing of tokens to experts and the plan the expert GEMMs read.
 //
-// Router (one warp per row, lane l holding experts l, l+32, ...): with logits
+// Router: with logits
 // x, scores s = softmax(x) or 1 / (1 + exp(-x)) over the experts that are open
 // (x > -inf), values v = s + bias, and, with groups, only the experts of the
 // groups with the greatest strength (the sum of a group's best one or two
@@ -21,17 +21,28 @@
 // matches.  No atomic decides an order, so the plan is the same on every run.
 // Up to kRouteRowsPerCta rows fit one CTA, which then does both.
 // The router reads rows * E logits and writes 16 bytes per pair.
+//
+// A CTA copies a tile of rows into shared memory (coalesced, transposed) and
+// gives each row L lanes, as many as it has threads for: one when the rows are
+// many, so that no instruction is spent on lanes agreeing, 32 for a few. Each
+// lane keeps the sorted best of its experts (i L + its number), then the lanes'
+// lists are merged. (A warp per row took 243 us for 90077 rows of 64 experts in
+// groups, 8 lanes a row with eight experts each in registers 80 us.)
 #include "common.cuh"
 #include "internal.h"
 
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 namespace tj {
 
-constexpr int kRouteThreads = 512;
+constexpr int kRouteThreads = 1024;
 constexpr int kRouteWarps = kRouteThreads / 32;
-constexpr int kRouteRowsPerCta = 32;
+constexpr int kPlanTile = 4096;  // pairs sorted at a time
+constexpr int kRouteRowsPerCta = 64;
 constexpr int kRouteMaxChunks = 148;  // one CTA per SM; also the rows of the histogram table
+constexpr uint16_t kNoChoice = 0xffff;
 constexpr int kRouteMaxExperts = 512;
 constexpr int kRouteMaxTopK = 32;
 constexpr int kRouteMaxGroups = 32;
@@ -57,6 +68,8 @@ struct RouteParams {
   const int32_t* row_count;
   int rows, chunk_rows, E, top_k;
   int sigmoid, groups, top_groups, group_top, renorm;
+  int wide;                     // rows are whole 16-byte loads
+  int tile_rows, lanes, pitch;  // of the router's tiles
   float weight_scale;
   int32_t* experts;  // [rows][top_k]
   float* weights;    // [rows][top_k]
@@ -66,30 +79,6 @@ struct RouteParams {
   int32_t* hist;     // plan: [chunks][E]
 };
 
-// ---- warp reductions --------------------------------------------------------
-// Unsigned keys ordered like the floats they come from (no NaN; -0 joined to +0).
-__device__ __forceinline__ uint32_t float_order(float x) {
-  const uint32_t b = __float_as_uint(x + 0.0f);
-  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
-}
-__device__ __forceinline__ float order_float(uint32_t k) {
-  return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k);
-}
-__device__ __forceinline__ float warp_max(float v) {
-  return order_float(__reduce_max_sync(0xffffffffu, float_order(v)));
-}
-__device__ __forceinline__ double warp_max(double v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
-template <typename V>
-__device__ __forceinline__ V warp_sum(V v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
 template <typename V>
 __device__ __forceinline__ V neg_inf();
 template <>
@@ -97,88 +86,53 @@ __device__ __forceinline__ float neg_inf<float>() { return __int_as_float(0xff80
 template <>
 __device__ __forceinline__ double neg_inf<double>() { return __longlong_as_double(0xfff0000000000000ll); }
 
-// Greatest of the warp's live values (bit i of `alive` = v[i]) and its expert,
-// the lowest index among equals; -inf and -1 when nothing is live.
-template <int VPL, typename V>
-__device__ __forceinline__ V route_best(const V (&v)[VPL], uint32_t alive, int lane, int* expert) {
-  V best = neg_inf<V>();
-  int bi = 0;
-#pragma unroll
-  for (int i = 0; i < VPL; ++i)
-    if (((alive >> i) & 1u) && v[i] > best) {
-      best = v[i];
-      bi = i;
-    }
-  const V top = warp_max(best);
-  const unsigned cand = (alive != 0u && best == top && top > neg_inf<V>()) ? (unsigned)(bi * 32 + lane) : 0xffffffffu;
-  const unsigned e = __reduce_min_sync(0xffffffffu, cand);
-  *expert = e == 0xffffffffu ? -1 : (int)e;
-  return top;
+// Reductions over the L lanes (a power of two) of a row.
+template <typename V>
+__device__ __forceinline__ V row_max(V v, int L) {
+  for (int o = L >> 1; o > 0; o >>= 1) {
+    const V u = __shfl_xor_sync(0xffffffffu, v, o);
+    v = u > v ? u : v;
+  }
+  return v;
 }
-
-// The row's choices from its values: lane j < top_k receives the j-th expert
-// (-1 when fewer are left).  Returns true if two values whose order matters
-// lie within 2 * err of each other (err bounds the error of each value).
-template <int VPL, typename V>
-__device__ bool route_select(const V (&v)[VPL], uint32_t alive, const RouteParams& p, int group_top, V err,
-                             int lane, int* mine) {
-  bool close = false;
-  if (p.groups > 1) {
-    const int per = p.E / p.groups;
-    V strength = neg_inf<V>();  // of group `lane`
-    for (int g = 0; g < p.groups; ++g) {
-      uint32_t in_g = 0;
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) {
-        const int e = i * 32 + lane;
-        in_g |= (e >= g * per && e < (g + 1) * per) ? (1u << i) : 0u;
-      }
-      in_g &= alive;
-      int e1, e2;
-      V s = route_best<VPL, V>(v, in_g, lane, &e1);
-      if (group_top == 2 && e1 >= 0) {
-        if ((e1 & 31) == lane) in_g &= ~(1u << (e1 >> 5));
-        const V s2 = route_best<VPL, V>(v, in_g, lane, &e2);
-        if (e2 >= 0) s += s2;
-      }
-      if (lane == g && e1 >= 0) strength = s;
-    }
-    // top_groups rounds over the lanes' strengths, then the best one left.
-    uint32_t kept = 0;
-    V worst = neg_inf<V>();
-    bool open = strength > neg_inf<V>();
-    for (int r = 0; r <= p.top_groups; ++r) {
-      const V s1[1] = {strength};
-      int g;
-      const V top = route_best<1, V>(s1, open ? 1u : 0u, lane, &g);
-      if (g < 0) break;
-      if (r == p.top_groups) {
-        close |= worst - top <= 6 * err;  // each strength is a rounded sum of up to two values
-        break;
-      }
-      kept |= 1u << g;
-      worst = top;
-      if (lane == g) open = false;
-    }
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      const int g = (i * 32 + lane) / per;
-      if (!((kept >> (g & 31)) & 1u)) alive &= ~(1u << i);
+template <typename V>
+__device__ __forceinline__ V row_sum(V v, int L) {
+  for (int o = L >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+// The greatest value and its expert, the lowest index among equals.
+template <typename V>
+__device__ __forceinline__ void row_best(V& v, int& e, int L) {
+  for (int o = L >> 1; o > 0; o >>= 1) {
+    const V u = __shfl_xor_sync(0xffffffffu, v, o);
+    const int f = __shfl_xor_sync(0xffffffffu, e, o);
+    if (u > v || (u == v && f < e)) {
+      v = u;
+      e = f;
     }
   }
-  V before = neg_inf<V>();
-  *mine = -1;
-  for (int r = 0; r <= p.top_k; ++r) {
-    int e;
-    const V top = route_best<VPL, V>(v, alive, lane, &e);
-    if (e < 0) break;
-    if (r > 0) close |= before - top <= 2 * err;
-    if (r == p.top_k) break;
-    if (lane == r) *mine = e;
-    if ((e & 31) == lane) alive &= ~(1u << (e >> 5));
-    before = top;
+}
+// The greatest two values, a >= b, -inf where there are fewer.
+__device__ __forceinline__ void push_top2(float& a, float& b, float x) {
+  b = fmaxf(b, fminf(a, x));
+  a = fmaxf(a, x);
+}
+__device__ __forceinline__ void push_top2(double& a, double& b, double x) {
+  b = fmax(b, fmin(a, x));
+  a = fmax(a, x);
+}
+template <typename V>
+__device__ __forceinline__ void row_top2(V& a, V& b, int L) {
+  for (int o = L >> 1; o > 0; o >>= 1) {
+    const V c = __shfl_xor_sync(0xffffffffu, a, o), d = __shfl_xor_sync(0xffffffffu, b, o);
+    push_top2(a, b, c);
+    push_top2(a, b, d);
   }
-  return close;
+}
+// A group's strength; -inf without an open expert.
+template <typename V>
+__device__ __forceinline__ V group_strength(V a, V b, int group_top) {
+  return group_top == 2 && b > neg_inf<V>() ? a + b : a;
 }
 
 template <typename T>
@@ -186,107 +140,307 @@ __device__ __forceinline__ float route_load(const T* p) {
   return (float)__ldg(p);
 }
 
-// One row: lane j < top_k receives expert and weight of choice j.
-template <int VPL, typename T>
-__device__ void route_row(const RouteParams& p, const float (&bias)[VPL], float bias_max, int row, int lane,
-                          int* mine, float* weight) {
-  const T* lg = static_cast<const T*>(p.logits) + (int64_t)row * p.E;
-  float x[VPL];
-  uint32_t alive = 0;
-  bool nan = false, pinf = false;
-  float m = neg_inf<float>();
-#pragma unroll
-  for (int i = 0; i < VPL; ++i) {
+// A row's choices in fp64, a warp to the row: lane j writes choice j.  m: the
+// row's greatest logit or 0.
+template <typename T>
+__device__ __noinline__ void route_row_exact(const RouteParams& p, const float* bias, const T* lg, float m, int lane,
+                                             uint16_t* chosen) {
+  constexpr int V = kRouteMaxExperts / 32;
+  const int n = (p.E + 31) / 32;  // of the V places used
+  double v[V];                    // of experts i * 32 + lane
+  double z = 0.0;
+  for (int i = 0; i < n; ++i) {
     const int e = i * 32 + lane;
-    x[i] = e < p.E ? route_load(lg + e) : neg_inf<float>();
+    const double x = e < p.E ? (double)route_load(lg + e) : neg_inf<double>();
+    v[i] = exp(p.sigmoid ? -x : x - (double)m);
+    z += v[i];
+    if (!(x > neg_inf<double>())) v[i] = neg_inf<double>();
   }
+  if (!p.sigmoid) z = row_sum(z, 32);
+  for (int i = 0; i < n; ++i) {
+    const int e = i * 32 + lane;
+    if (v[i] > neg_inf<double>())
+      v[i] = (p.sigmoid ? 1.0 / (1.0 + v[i]) : v[i] / z) + (double)(p.bias ? bias[e] : 0.f);
+  }
+  if (p.groups > 1) {
+    const int per = p.E / p.groups;
+    double strength = neg_inf<double>();  // of group `lane`
+    for (int g = 0; g < p.groups; ++g) {
+      double a = neg_inf<double>(), b = neg_inf<double>();
+      for (int i = 0; i < n; ++i) {
+        const int e = i * 32 + lane;
+        push_top2(a, b, e >= g * per && e < (g + 1) * per ? v[i] : neg_inf<double>());
+      }
+      row_top2(a, b, 32);
+      if (lane == g) strength = group_strength(a, b, p.group_top);
+    }
+    int above = 0;
+    for (int g = 0; g < p.groups; ++g) {
+      const double o = __shfl_sync(0xffffffffu, strength, g);
+      above += o > strength || (o == strength && g < lane);
+    }
+    const unsigned kept = __ballot_sync(0xffffffffu, lane < p.groups && above < p.top_groups);
+    for (int i = 0; i < n; ++i)
+      if (!((kept >> (((i * 32 + lane) / per) & 31)) & 1u)) v[i] = neg_inf<double>();
+  }
+  for (int j = 0; j < p.top_k; ++j) {
+    double best = neg_inf<double>();
+    int e = lane;
+    for (int i = 0; i < n; ++i)
+      if (v[i] > best) {
+        best = v[i];
+        e = i * 32 + lane;
+      }
+    row_best(best, e, 32);
+    for (int i = 0; i < n; ++i)
+      if (e == i * 32 + lane) v[i] = neg_inf<double>();
+    if (lane == 0) chosen[j] = best > neg_inf<double>() ? (uint16_t)e : kNoChoice;
+  }
+}
+
+// The KL greatest values pushed, descending, earlier ones first among equals,
+// and the greatest of the rest.
+template <int KL>
+struct RouteList {
+  float v[KL];
+  int e[KL];
+  float rest;
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-  for (int i = 0; i < VPL; ++i) {
-    nan |= isnan(x[i]);
-    pinf |= x[i] == -neg_inf<float>();
-    if (x[i] > neg_inf<float>()) {
-      alive |= 1u << i;
-      m = fmaxf(m, x[i]);
+    for (int i = 0; i < KL; ++i) {
+      v[i] = neg_inf<float>();
+      e[i] = 0;
+    }
+    rest = neg_inf<float>();
+  }
+  __device__ __forceinline__ void push(float x, int f) {
+    if (!(x > v[KL - 1])) {
+      rest = fmaxf(rest, x);
+      return;
+    }
+    rest = fmaxf(rest, v[KL - 1]);
+#pragma unroll
+    for (int i = KL - 1; i > 0; --i) {
+      const bool here = x > v[i], before = x > v[i - 1];
+      v[i] = here ? (before ? v[i - 1] : x) : v[i];
+      e[i] = here ? (before ? e[i - 1] : f) : e[i];
+    }
+    if (x > v[0]) {
+      v[0] = x;
+      e[0] = f;
     }
   }
-  // A row whose scores are not numbers is chosen by its logits and has NaN weights.
-  const bool bad = __any_sync(0xffffffffu, nan || (pinf && !p.sigmoid));
-  const bool by_value = !bad && (p.bias != nullptr || (p.groups > 1 && p.group_top == 2));
-  const bool need_sum = !p.sigmoid && (by_value || !p.renorm);
-  m = warp_max(m);
-  float z = 0.f;
-  if (need_sum) {
+  __device__ __forceinline__ void pop() {
 #pragma unroll
-    for (int i = 0; i < VPL; ++i)
-      if ((alive >> i) & 1u) z += expf(x[i] - m);
-    z = warp_sum(z);
+    for (int i = 0; i + 1 < KL; ++i) {
+      v[i] = v[i + 1];
+      e[i] = e[i + 1];
+    }
+    v[KL - 1] = neg_inf<float>();
   }
-  if (!by_value) {
-    route_select<VPL, float>(x, alive, p, 1, -1.f, lane, mine);
+};
+
+// One tile: rows [t0, t0 + n) in shared memory, xs[e * pitch + row]; flags[row]
+// set for a row whose scores are not numbers.  Thread = (row, lane of L).
+// Writes the choices to chosen[row * top_k + j] and, by the row's lane 0,
+// top[row], zs[row] for the weights.  All threads of a warp take part.
+template <int KL, typename T>
+__device__ void route_choose(const RouteParams& p, const float* bias, float bias_max, float* xs, int pitch,
+                             const int* flags, float* strengths, float* tops, float* zs, uint16_t* chosen, int t0,
+                             int n, int L) {
+  const int row = (int)threadIdx.x / L, sub = (int)threadIdx.x & (L - 1), lane = (int)threadIdx.x & 31;
+  const bool on = row < n;
+  const int E = p.E;
+  float* x = xs + (on ? row : 0);
+  const bool bad = on && flags[row] != 0;
+  const bool by_value = p.bias != nullptr || (p.groups > 1 && p.group_top == 2);
+  float top = 0.f, z = 1.f;
+  if (!p.sigmoid && (by_value || !p.renorm)) {
+    float m = neg_inf<float>();
+#pragma unroll 4
+    for (int e = sub; e < E; e += L) m = fmaxf(m, x[e * pitch]);
+    m = row_max(m, L);
+    top = m > neg_inf<float>() ? m : 0.f;  // a closed row's exponentials are 0, not NaN
+    z = 0.f;
+#pragma unroll 4
+    for (int e = sub; e < E; e += L) z += expf(x[e * pitch] - top);
+    z = row_sum(z, L);
+  }
+  const float zi = 1.f / z;
+  float err = -1.f;  // the logits themselves: no two are too close
+  if (by_value && !bad) {
+    // |error of v| <= |error of s| + 2^-24 |v|.  Sigmoid: e = 2^(-x log2 e) with
+    // the product rounded (|x| 2^-23 relative) and ex2 within 2 ulp, 1 + e rounded,
+    // the quotient within 2 ulp: s (1 - s) (2^-22 + |x| 2^-23) + s (2^-24 + 2^-22),
+    // at most 4.2e-7.  Softmax: the sum of up to 512 terms (at most 64 in order,
+    // then the lanes) is within 69 ulp (2^-24 each), expf within 2 ulp, two more
+    // roundings: 5e-6 of the greatest score, 1 / z.
+    const float smax = p.sigmoid ? 1.f : zi;
+    err = (p.sigmoid ? 4.2e-7f : 5e-6f * smax) + 6e-8f * (smax + bias_max);
+  }
+  // Value of expert e, in place of its logit.
+  const bool set = by_value && on && !bad;
+  auto value = [&](int e) {
+    const float a = x[e * pitch];
+    if (!by_value) return a;
+    const float sc = p.sigmoid ? __fdividef(1.f, 1.f + __expf(-a)) : expf(a - top) * zi;
+    float v = sc + (p.bias ? bias[e] : 0.f);
+    v = a > neg_inf<float>() ? v : neg_inf<float>();
+    v = bad ? a : v;
+    if (set) x[e * pitch] = v;
+    return v;
+  };
+  bool close = false;
+  uint32_t kept = 0xffffffffu;
+  const int per = E / p.groups;
+  if (p.groups > 1) {
+    const int group_top = bad ? 1 : p.group_top;
+    float* st = strengths + (on ? row : 0);  // [group * pitch]
+    for (int g = 0; g < p.groups; ++g) {
+      float a = neg_inf<float>(), b = neg_inf<float>();
+#pragma unroll 4
+      for (int e = g * per + ((sub - g * per) & (L - 1)); e < (g + 1) * per; e += L) push_top2(a, b, value(e));
+      row_top2(a, b, L);
+      if (on && sub == 0) st[g * pitch] = group_strength(a, b, group_top);
+    }
+    __syncwarp();
+    float weakest = -neg_inf<float>(), dropped = neg_inf<float>();
+    kept = 0;
+    for (int g = sub; g < p.groups; g += L) {
+      const float s = st[g * pitch];
+      int above = 0;
+#pragma unroll 4
+      for (int h = 0; h < p.groups; ++h) {
+        const float o = st[h * pitch];
+        above += o > s || (o == s && h < g);
+      }
+      if (above < p.top_groups) {
+        kept |= 1u << g;
+        if (s > neg_inf<float>()) weakest = fminf(weakest, s);
+      } else {
+        dropped = fmaxf(dropped, s);
+      }
+    }
+    for (int o = L >> 1; o > 0; o >>= 1) kept |= __shfl_xor_sync(0xffffffffu, kept, o);
+    weakest = -row_max(-weakest, L);
+    dropped = row_max(dropped, L);
+    // a strength is a rounded sum of up to two values
+    close = dropped > neg_inf<float>() && weakest - dropped <= 6 * err;
+  }
+  RouteList<KL> list;
+  list.clear();
+  if (p.groups > 1) {
+    // only the groups kept, each row its own, in index order
+    for (int i = 0; i < p.top_groups; ++i) {
+      const int g = __ffs(kept) - 1;
+      kept &= kept - 1;
+      const int e0 = g * per;
+#pragma unroll 2
+      for (int e = e0 + ((sub - e0) & (L - 1)); e < e0 + per; e += L) list.push(x[e * pitch], e);
+    }
   } else {
-    float v[VPL];
-    uint32_t live = alive;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      const float s = p.sigmoid ? 1.f / (1.f + expf(-x[i])) : expf(x[i] - m) / z;
-      v[i] = s + bias[i];
-      if (!(v[i] > neg_inf<float>())) live &= ~(1u << i);  // closed by its bias (or NaN)
-    }
-    // |error of v| <= 2e-6 max(s) + 2^-24 |v|: expf within 2 ulp, the sum of
-    // up to 512 terms (16 in order, then 5 levels) within 21 ulp, division and
-    // addition within half an ulp each; max(s) is 1/z or at most 1.
-    const float smax = p.sigmoid ? 1.f : 1.f / z;
-    const float err = 2e-6f * smax + 1.2e-7f * (smax + bias_max);
-    if (route_select<VPL, float>(v, live, p, p.group_top, err, lane, mine)) {
-      double zd = 0.0;
-      if (!p.sigmoid) {
-#pragma unroll 1
-        for (int i = 0; i < VPL; ++i)
-          if ((alive >> i) & 1u) zd += exp((double)x[i] - (double)m);
-        zd = warp_sum(zd);
-      }
-      double vd[VPL];
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) {
-        const double a = p.sigmoid ? exp(-(double)x[i]) : exp((double)x[i] - (double)m);
-        vd[i] = (p.sigmoid ? 1.0 / (1.0 + a) : a / zd) + (double)bias[i];
-      }
-      route_select<VPL, double>(vd, live, p, p.group_top, -1.0, lane, mine);
-    }
+#pragma unroll 2
+    for (int e = sub; e < E; e += L) list.push(value(e), e);
   }
-  // Weights: lane j holds choice j.
-  const bool have = *mine >= 0;
-  const float c = have ? route_load(lg + *mine) : neg_inf<float>();
-  float w = 0.f;
-  if (p.sigmoid) {
-    w = have ? 1.f / (1.f + expf(-c)) : 0.f;
-    if (p.renorm) {
-      float sum = warp_sum(w);
-      if (sum < 1e-30f) {  // far below zero the scores underflow, their ratios do not
-        const float cm = warp_max(c);
-        w = have ? expf(c - cm) : 0.f;
-        sum = warp_sum(w);
+  // Merge: the best head of the lanes' lists, top_k times.
+  float before = -neg_inf<float>();
+  uint16_t* out = chosen + (on ? row : 0) * p.top_k;
+  if (L == 1) {
+#pragma unroll
+    for (int j = 0; j < KL; ++j)
+      if (j < p.top_k) {
+        const bool found = list.v[j] > neg_inf<float>();
+        close |= found && before - list.v[j] <= 2 * err;  // inf - inf compares false
+        before = list.v[j];
+        if (on) out[j] = found ? (uint16_t)list.e[j] : kNoChoice;
+      } else {
+        list.rest = fmaxf(list.rest, list.v[j]);
       }
-      w = sum > 0.f ? w / sum : 0.f;
-    }
-  } else if (p.renorm) {
-    // the denominator of the softmax cancels
-    const float cm = warp_max(c);
-    w = have ? expf(c - cm) : 0.f;
-    const float sum = warp_sum(w);
-    w = sum > 0.f ? w / sum : 0.f;
   } else {
-    w = have ? expf(c - m) / z : 0.f;
+    for (int j = 0; j < p.top_k; ++j) {
+      float v = list.v[0];
+      int e = list.e[0];
+      row_best(v, e, L);
+      const bool found = v > neg_inf<float>();
+      close |= found && before - v <= 2 * err;
+      before = v;
+      if (found && (e & (L - 1)) == sub) list.pop();
+      if (on && sub == 0) out[j] = found ? (uint16_t)e : kNoChoice;
+    }
+    list.rest = row_max(fmaxf(list.rest, list.v[0]), L);
   }
-  *weight = bad ? __int_as_float(0x7fc00000) : w * p.weight_scale;
+  close |= list.rest > neg_inf<float>() && before - list.rest <= 2 * err;
+  if (on && sub == 0) {
+    tops[row] = top;
+    zs[row] = z;
+  }
+  __syncwarp();
+  // Rows too close to call in fp32, the whole warp at each.
+  for (unsigned again = __ballot_sync(0xffffffffu, close && on && sub == 0); again != 0; again &= again - 1) {
+    const int r = ((int)threadIdx.x - lane + __ffs(again) - 1) / L;
+    route_row_exact<T>(p, bias, static_cast<const T*>(p.logits) + (int64_t)(t0 + r) * E, tops[r], lane,
+                       chosen + r * p.top_k);
+  }
+  __syncwarp();
+}
+
+// The weights of a tile's choices, L lanes to a row, lane j, j + L, ... of them.
+template <typename T>
+__device__ void route_weights(const RouteParams& p, const int* flags, const float* tops, const float* zs,
+                              const uint16_t* chosen, int t0, int n, int live, int L) {
+  const int row = (int)threadIdx.x / L, sub = (int)threadIdx.x & (L - 1);
+  const bool on = row < n;
+  const int64_t grow = t0 + (on ? row : 0);
+  const T* lg = static_cast<const T*>(p.logits) + grow * p.E;
+  const uint16_t* mine = chosen + (on ? row : 0) * p.top_k;
+  const bool here = on && grow < live;
+  const float top = on ? tops[row] : 0.f, z = on ? zs[row] : 1.f;
+  float cm = neg_inf<float>(), sum = 0.f, near = 0.f;
+  if (p.renorm) {
+    if (here)
+#pragma unroll 4
+      for (int j = sub; j < p.top_k; j += L)
+        if (mine[j] != kNoChoice) cm = fmaxf(cm, route_load(lg + mine[j]));
+    cm = row_max(cm, L);
+    if (!(cm > neg_inf<float>())) cm = 0.f;
+    if (here)
+#pragma unroll 4
+      for (int j = sub; j < p.top_k; j += L)
+        if (mine[j] != kNoChoice) {
+          const float c = route_load(lg + mine[j]);
+          near += expf(c - cm);  // softmax: its denominator cancels
+          if (p.sigmoid) sum += 1.f / (1.f + expf(-c));
+        }
+    near = row_sum(near, L);
+    sum = row_sum(sum, L);
+  }
+  // Far below zero the sigmoids underflow, their ratios (those of exp) do not.
+  const bool ratio = p.renorm && (!p.sigmoid || sum < 1e-30f);
+  const float scale = !p.renorm ? p.weight_scale : (ratio ? (near > 0.f ? p.weight_scale / near : 0.f) : p.weight_scale / sum);
+  const bool bad = here && flags[row] != 0;
+  if (on)
+#pragma unroll 4
+    for (int j = sub; j < p.top_k; j += L) {
+      const int e = here && mine[j] != kNoChoice ? mine[j] : -1;
+      float w = 0.f;
+      if (e >= 0) {
+        const float c = route_load(lg + e);
+        w = ratio ? expf(c - cm) : (p.sigmoid ? 1.f / (1.f + expf(-c)) : expf(c - top) / z);
+      }
+      p.experts[grow * p.top_k + j] = e;
+      p.weights[grow * p.top_k + j] = bad ? __int_as_float(0x7fc00000) : w * scale;
+    }
 }
 
 // ---- plan ---------------------------------------------------------------------
-// An expert index of the choices, -1 for none (or out of range).
-__device__ __forceinline__ int plan_expert(const RouteParams& p, int64_t item, int64_t live_items) {
-  if (item >= live_items) return -1;
-  const int e = p.experts[item];
-  return (e >= 0 && e < p.E) ? e : -1;
+
+// Shared memory of the sort, after `vectors` arrays of E ints.
+__device__ __forceinline__ int* plan_runs(int* smem, int vectors, int E) { return smem + vectors * E; }
+__device__ __forceinline__ uint16_t* plan_tile(int* smem, int vectors, int E) {
+  return reinterpret_cast<uint16_t*>(smem + (vectors + ((int)blockDim.x >> 5)) * E);
+}
+static size_t plan_smem(int vectors, int warps, int E) {
+  return (size_t)(vectors + warps) * E * sizeof(int) + kPlanTile * sizeof(uint16_t);
 }
 
 // Exclusive scan of v[0..n) in place by one warp; returns the total.
@@ -306,104 +460,170 @@ __device__ int warp_scan_exclusive(int* v, int n, int lane) {
   return carry;
 }
 
-// Slots of this CTA's pairs (rows [r0, r1)).  base[e]: first slot of the
-// chunk's pairs of expert e.  whist: [kRouteWarps][E] ints of shared memory.
-// Each warp owns a run of pairs, so ranks inside a warp (matches) and the
-// counts of the warps before it give the rank in (row, j) order.
-__device__ void plan_scatter(const RouteParams& p, int r0, int r1, int64_t live_items, const int* base, int* whist) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t i0 = (int64_t)r0 * p.top_k, i1 = (int64_t)r1 * p.top_k;
-  const int64_t run = ((i1 - i0 + kRouteThreads - 1) / kRouteThreads) * 32;
-  const int64_t w0 = min(i0 + warp * run, i1), w1 = min(w0 + run, i1);
-  for (int i = threadIdx.x; i < kRouteWarps * p.E; i += kRouteThreads) whist[i] = 0;
+// Slots of the `n` pairs from pair i0 whose experts lie in `tile` (kNoChoice:
+// none).  base[e]: next slot of expert e, advanced past these pairs.  Each warp
+// owns a run of pairs, so ranks inside a warp (matches) and the counts of the
+// warps before it (runs: [warps][E]) give the rank in (row, j) order.
+__device__ void plan_sort(const RouteParams& p, int i0, int n, const uint16_t* tile, int* base, int* runs) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = (int)blockDim.x >> 5;
+  const int run = (n + 32 * warps - 1) / (32 * warps) * 32;
+  const int w0 = min(warp * run, n), w1 = min(w0 + run, n);
+  for (int i = threadIdx.x; i < warps * p.E; i += (int)blockDim.x) runs[i] = 0;
   __syncthreads();
-  int* mine = whist + warp * p.E;
-  for (int64_t i = w0 + lane; i < w1; i += 32) {
-    const int e = plan_expert(p, i, live_items);
-    if (e >= 0) atomicAdd(mine + e, 1);
-  }
+  int* mine = runs + warp * p.E;
+  for (int i = w0 + lane; i < w1; i += 32)
+    if (tile[i] != kNoChoice) atomicAdd(mine + tile[i], 1);
   __syncthreads();
-  for (int e = threadIdx.x; e < p.E; e += kRouteThreads) {
+  for (int e = threadIdx.x; e < p.E; e += (int)blockDim.x) {
     int at = base[e];
-#pragma unroll 1
-    for (int w = 0; w < kRouteWarps; ++w) {
-      const int n = whist[w * p.E + e];
-      whist[w * p.E + e] = at;
-      at += n;
+#pragma unroll 8
+    for (int w = 0; w < warps; ++w) {
+      const int c = runs[w * p.E + e];
+      runs[w * p.E + e] = at;
+      at += c;
     }
+    base[e] = at;
   }
   __syncthreads();
-  for (int64_t b = w0; b < w1; b += 32) {
-    const int64_t i = b + lane;
-    const int e = i < w1 ? plan_expert(p, i, live_items) : -1;
+  for (int b = w0; b < w1; b += 32) {
+    const int i = b + lane;
+    const int e = i < w1 ? tile[i] : kNoChoice;
     const unsigned same = __match_any_sync(0xffffffffu, e);
     const int rank = __popc(same & ((1u << lane) - 1u));
-    const int at = e >= 0 ? mine[e] + rank : -1;
+    const int at = e != kNoChoice ? mine[e] + rank : -1;
     __syncwarp();
-    if (e >= 0 && rank == 0) mine[e] += __popc(same);
+    if (e != kNoChoice && rank == 0) mine[e] += __popc(same);
     __syncwarp();
     if (i < w1) {
-      p.row_slot[i] = at;
-      if (at >= 0) p.slot_row[at] = (int32_t)(i / p.top_k);
+      p.row_slot[i0 + i] = at;
+      if (at >= 0) p.slot_row[at] = (int)((unsigned)(i0 + i) / (unsigned)p.top_k);
     }
   }
+  __syncthreads();  // the next tile rewrites the runs
 }
 
 // slot_row of the slots no pair has, split over the CTAs.
 __device__ void plan_fill_unused(const RouteParams& p, int used) {
   const int64_t n = (int64_t)p.rows * p.top_k;
-  for (int64_t i = used + (int64_t)blockIdx.x * kRouteThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kRouteThreads)
-    p.slot_row[i] = -1;
+  const int64_t step = (int64_t)gridDim.x * blockDim.x;
+  for (int64_t i = used + (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += step) p.slot_row[i] = -1;
 }
 
 // Router over one chunk of rows per CTA (or, without logits, a check of the
 // given choices) and the chunk's histogram; with one chunk, the plan too.
-// Dynamic shared memory: (kRouteWarps + 2) * E ints.
-template <int VPL, typename T>
-__global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams p) {
+// Dynamic shared memory: plan_smem(2, warps, E), then the tile: logits and
+// strengths [(E + groups) * pitch], flags, tops and zs [tile_rows].  KL: 0
+// without logits.
+template <int KL, typename T>
+__global__ void __launch_bounds__(KL > 16 ? 512 : kRouteThreads) route_kernel(const RouteParams p) {
   extern __shared__ int route_smem[];
-  int* hist = route_smem;             // [E]
-  int* whist = route_smem + p.E;      // [kRouteWarps][E]
+  int* hist = route_smem;                                      // [E]
+  float* bias = reinterpret_cast<float*>(route_smem + p.E);    // [E]
+  uint16_t* tile = plan_tile(route_smem, 2, p.E);              // choices: of the chunk if it is the only one
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int i = threadIdx.x; i < p.E; i += kRouteThreads) hist[i] = 0;
-  __syncthreads();
+  const bool alone = gridDim.x == 1;
+  for (int i = threadIdx.x; i < p.E; i += (int)blockDim.x) hist[i] = 0;
+  if (alone) pdl_trigger();  // the other SMs set up what follows meanwhile
   pdl_wait();
   const int live = p.row_count ? max(0, min(p.rows, *p.row_count)) : p.rows;
   const int r0 = (int)min((int64_t)blockIdx.x * p.chunk_rows, (int64_t)p.rows);
   const int r1 = (int)min((int64_t)r0 + p.chunk_rows, (int64_t)p.rows);
-  const int64_t live_items = (int64_t)live * p.top_k;
-  if (p.logits != nullptr) {
-    float bias[VPL];
+  if constexpr (KL > 0) {
+    float* xs = reinterpret_cast<float*>(tile + kPlanTile);
+    float* strengths = xs + p.E * p.pitch;
+    int* flags = reinterpret_cast<int*>(strengths + (p.groups > 1 ? p.groups * p.pitch : 0));
+    float* tops = reinterpret_cast<float*>(flags + p.tile_rows);
+    float* zs = tops + p.tile_rows;
     float bias_max = 0.f;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      const int e = i * 32 + lane;
-      bias[i] = (p.bias && e < p.E) ? __ldg(p.bias + e) : 0.f;
-      if (fabsf(bias[i]) < -neg_inf<float>()) bias_max = fmaxf(bias_max, fabsf(bias[i]));
-    }
-    bias_max = warp_max(bias_max);
-    for (int row = r0 + warp; row < r1; row += kRouteWarps) {
-      int mine = -1;
-      float w = 0.f;
-      if (row < live) route_row<VPL, T>(p, bias, bias_max, row, lane, &mine, &w);
-      if (lane < p.top_k) {
-        p.experts[(int64_t)row * p.top_k + lane] = mine;
-        p.weights[(int64_t)row * p.top_k + lane] = w;
-        if (mine >= 0) atomicAdd(hist + mine, 1);
+    if (p.bias) {
+      for (int i = threadIdx.x; i < p.E; i += (int)blockDim.x) {
+        const float b = __ldg(p.bias + i);
+        bias[i] = isnan(b) ? neg_inf<float>() : b;  // closed by its bias
       }
+      for (int i = lane; i < p.E; i += 32) {
+        const float b = fabsf(__ldg(p.bias + i));
+        if (b < -neg_inf<float>()) bias_max = fmaxf(bias_max, b);
+      }
+      bias_max = row_max(bias_max, 32);
+    }
+    for (int t0 = r0; t0 < r1; t0 += p.tile_rows) {
+      const int n = min(p.tile_rows, r1 - t0);
+      uint16_t* chosen = alone ? tile + (t0 - r0) * p.top_k : tile;
+      for (int i = threadIdx.x; i < n; i += (int)blockDim.x) flags[i] = 0;
+      __syncthreads();
+      // Rows in order, elements in order: coalesced, and with an odd pitch no
+      // two lanes write one bank.  Rows that are not live are closed.
+      const T* from = static_cast<const T*>(p.logits) + (int64_t)t0 * p.E;
+      const int items = n * p.E, read = max(0, min(live - t0, n)) * p.E;
+      // W values to a load, when rows are whole loads.
+      auto stage = [&](auto width) {
+        constexpr int W = decltype(width)::value;
+        const int units = p.E / W;  // of a row
+        int row = (int)threadIdx.x / units, u = (int)threadIdx.x % units;
+        const int row_step = (int)blockDim.x / units, u_step = (int)blockDim.x % units;
+#pragma unroll 4
+        for (int i = (int)threadIdx.x * W; i < items; i += (int)blockDim.x * W) {
+          float x[W];
+          if (i < read) {
+            if constexpr (W > 1) {
+              alignas(16) T t[W];
+              *reinterpret_cast<uint4*>(t) = __ldg(reinterpret_cast<const uint4*>(from + i));
+#pragma unroll
+              for (int k = 0; k < W; ++k) x[k] = (float)t[k];
+            } else {
+              x[0] = route_load(from + i);
+            }
+            float odd = 0.f;
+#pragma unroll
+            for (int k = 0; k < W; ++k) odd = fmaf(x[k], 0.f, odd);
+            if (odd != 0.f) {  // NaN: some value is NaN or infinite
+#pragma unroll
+              for (int k = 0; k < W; ++k) {
+                if (isnan(x[k]) || (x[k] == -neg_inf<float>() && !p.sigmoid)) flags[row] = 1;
+                if (isnan(x[k])) x[k] = neg_inf<float>();
+              }
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < W; ++k) x[k] = neg_inf<float>();
+          }
+#pragma unroll
+          for (int k = 0; k < W; ++k) xs[(u * W + k) * p.pitch + row] = x[k];
+          row += row_step;
+          u += u_step;
+          if (u >= units) {
+            u -= units;
+            ++row;
+          }
+        }
+      };
+      if (p.wide)
+        stage(std::integral_constant<int, 16 / sizeof(T)>());
+      else
+        stage(std::integral_constant<int, 1>());
+      __syncthreads();
+      route_choose<KL, T>(p, bias, bias_max, xs, p.pitch, flags, strengths, tops, zs, chosen, t0, n, p.lanes);
+      route_weights<T>(p, flags, tops, zs, chosen, t0, n, live, p.lanes);
+      __syncthreads();
+      for (int i = threadIdx.x; i < n * p.top_k; i += (int)blockDim.x)
+        if (chosen[i] != kNoChoice) atomicAdd(hist + chosen[i], 1);
+      __syncthreads();
     }
   } else {
-    const int64_t i1 = min((int64_t)r1 * p.top_k, live_items);
-    for (int64_t i = (int64_t)r0 * p.top_k + threadIdx.x; i < i1; i += kRouteThreads) {
-      const int e = p.experts[i];
+    const int64_t i0 = (int64_t)r0 * p.top_k, i1 = (int64_t)r1 * p.top_k, on = (int64_t)live * p.top_k;
+    __syncthreads();
+    for (int64_t i = i0 + threadIdx.x; i < i1; i += blockDim.x) {
+      const int e = i < on ? p.experts[i] : -1;
       if (e >= p.E) report_error(kDevBadArgument, 240);
-      if (e >= 0 && e < p.E) atomicAdd(hist + e, 1);
+      const bool in = e >= 0 && e < p.E;
+      if (in) atomicAdd(hist + e, 1);
+      if (alone) tile[i - i0] = in ? (uint16_t)e : kNoChoice;
     }
   }
   __syncthreads();
-  if (gridDim.x > 1) {
+  if (!alone) {
     pdl_trigger();
-    for (int i = threadIdx.x; i < p.E; i += kRouteThreads) p.hist[(int64_t)blockIdx.x * p.E + i] = hist[i];
+    for (int i = threadIdx.x; i < p.E; i += (int)blockDim.x) p.hist[(int64_t)blockIdx.x * p.E + i] = hist[i];
     return;
   }
   __shared__ int used;
@@ -412,27 +632,28 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams 
     if (lane == 0) used = n;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i <= p.E; i += kRouteThreads) p.offsets[i] = i < p.E ? hist[i] : used;
+  for (int i = threadIdx.x; i <= p.E; i += (int)blockDim.x) p.offsets[i] = i < p.E ? hist[i] : used;
   plan_fill_unused(p, used);
-  plan_scatter(p, r0, r1, live_items, hist, whist);
+  plan_sort(p, 0, p.rows * p.top_k, tile, hist, plan_runs(route_smem, 2, p.E));  // at most kPlanTile pairs
 }
 
-// Plan of several chunks.  Dynamic shared memory: (kRouteWarps + 2) * E ints.
+// Plan of several chunks.  Dynamic shared memory: plan_smem(2, warps, E).
 __global__ void __launch_bounds__(kRouteThreads) expert_plan_kernel(const RouteParams p) {
   extern __shared__ int route_smem[];
   int* total = route_smem;           // [E], then its exclusive scan
   int* base = route_smem + p.E;      // [E] pairs of the chunks before this one
-  int* whist = route_smem + 2 * p.E;
+  uint16_t* tile = plan_tile(route_smem, 2, p.E);
   __shared__ int used;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int i = threadIdx.x; i < 2 * p.E; i += kRouteThreads) route_smem[i] = 0;
   __syncthreads();
   pdl_wait();
   // Thread group q of E consecutive threads sums chunks q, q + groups, ...
-  const int groups = p.E < kRouteThreads ? kRouteThreads / p.E : 1;
-  for (int e = threadIdx.x; e < p.E * groups; e += kRouteThreads) {
-    const int ex = e % p.E, q = e / p.E;
+  const int groups = kRouteThreads / p.E;
+  if ((int)threadIdx.x < p.E * groups) {
+    const int ex = (int)threadIdx.x % p.E, q = (int)threadIdx.x / p.E;
     int all = 0, before = 0;
+#pragma unroll 8
     for (int c = q; c < (int)gridDim.x; c += groups) {
       const int n = __ldcg(p.hist + (int64_t)c * p.E + ex);
       all += n;
@@ -451,25 +672,90 @@ __global__ void __launch_bounds__(kRouteThreads) expert_plan_kernel(const RouteP
     for (int i = threadIdx.x; i <= p.E; i += kRouteThreads) p.offsets[i] = i < p.E ? total[i] : used;
   for (int i = threadIdx.x; i < p.E; i += kRouteThreads) base[i] += total[i];
   plan_fill_unused(p, used);
-  __syncthreads();
   const int live = p.row_count ? max(0, min(p.rows, *p.row_count)) : p.rows;
   const int r0 = (int)min((int64_t)blockIdx.x * p.chunk_rows, (int64_t)p.rows);
   const int r1 = (int)min((int64_t)r0 + p.chunk_rows, (int64_t)p.rows);
-  plan_scatter(p, r0, r1, (int64_t)live * p.top_k, base, whist);
+  const int i0 = r0 * p.top_k, i1 = r1 * p.top_k, on = min(live * p.top_k, i1);
+  for (int b = i0; b < i1; b += kPlanTile) {
+    const int n = min(kPlanTile, i1 - b);
+#pragma unroll
+    for (int u = 0; u < kPlanTile / kRouteThreads; ++u) {
+      const int i = u * kRouteThreads + (int)threadIdx.x;
+      if (i < n) {
+        const int e = b + i < on ? p.experts[b + i] : -1;
+        tile[i] = e >= 0 && e < p.E ? (uint16_t)e : kNoChoice;
+      }
+    }
+    __syncthreads();
+    plan_sort(p, b, n, tile, base, plan_runs(route_smem, 2, p.E));
+  }
 }
 
-template <int VPL, typename T>
-static cudaError_t launch_route_t(const RouteParams& p, int chunks, size_t smem, cudaStream_t stream) {
-  return launch_pdl(route_kernel<VPL, T>, dim3(chunks), dim3(kRouteThreads), smem, stream, p);
+constexpr size_t kRouteMaxSmem = 226 * 1024;  // with the static part, below 227 KB
+
+// Rows of a tile and lanes of a row: as many rows of the chunk as fit (with the
+// sort's part of shared memory, and the tile's choices in kPlanTile places),
+// in equal tiles, then as many lanes as the threads allow and the experts need.
+static void route_tile(RouteParams* p, int max_threads) {
+  const size_t fixed = plan_smem(2, kRouteWarps, p->E) + 64;
+  const size_t per_row = (size_t)(p->E + (p->groups > 1 ? p->groups : 0)) * 4 + 12;
+  int64_t rows = (int64_t)((kRouteMaxSmem - fixed) / per_row) - 2;  // - 2: the pitch is odd
+  rows = min(rows, (int64_t)max_threads);
+  rows = min(rows, (int64_t)kPlanTile / p->top_k);
+  rows = min(rows, (int64_t)p->chunk_rows);
+  const int64_t tiles = (p->chunk_rows + rows - 1) / rows;
+  p->tile_rows = (int)((p->chunk_rows + tiles - 1) / tiles);
+  p->pitch = p->tile_rows | 1;
+  int lanes = 1;
+  while (2 * lanes <= 32 && 2 * lanes * p->tile_rows <= max_threads && lanes < p->E) lanes *= 2;
+  p->lanes = lanes;
+}
+
+template <int KL, typename T>
+static cudaError_t launch_route_t(RouteParams p, int chunks, cudaStream_t stream) {
+  constexpr int kMost = KL > 16 ? 512 : kRouteThreads;
+  int threads = kMost;
+  size_t tile_bytes = 0;
+  if (KL > 0) {
+    route_tile(&p, kMost);
+    threads = (p.tile_rows * p.lanes + 31) / 32 * 32;
+    if (threads < 128) threads = 128;
+    tile_bytes = ((size_t)(p.E + (p.groups > 1 ? p.groups : 0)) * p.pitch + 3 * (size_t)p.tile_rows) * 4;
+  } else if (chunks == 1) {
+    threads = p.rows * p.top_k <= 256 ? 128 : kMost;
+  }
+  const size_t smem = plan_smem(2, threads / 32, p.E) + tile_bytes;
+  static bool attr_set[64] = {};
+  const int dev = device_index();
+  if (!attr_set[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(route_kernel<KL, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)kRouteMaxSmem);
+    if (e != cudaSuccess) return e;
+    attr_set[dev] = true;
+  }
+  return launch_pdl(route_kernel<KL, T>, dim3(chunks), dim3(threads), smem, stream, p);
+}
+
+static cudaError_t launch_plan(const RouteParams& p, int chunks, cudaStream_t stream) {
+  static bool attr_set[64] = {};
+  const int dev = device_index();
+  if (!attr_set[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(expert_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)plan_smem(2, kRouteWarps, kRouteMaxExperts));
+    if (e != cudaSuccess) return e;
+    attr_set[dev] = true;
+  }
+  return launch_pdl(expert_plan_kernel, dim3(chunks), dim3(kRouteThreads), plan_smem(2, kRouteWarps, p.E), stream, p);
 }
 
 template <typename T>
-static cudaError_t launch_route_vpl(const RouteParams& p, int chunks, size_t smem, cudaStream_t stream) {
-  if (p.E <= 32 || p.logits == nullptr) return launch_route_t<1, T>(p, chunks, smem, stream);
-  if (p.E <= 64) return launch_route_t<2, T>(p, chunks, smem, stream);
-  if (p.E <= 128) return launch_route_t<4, T>(p, chunks, smem, stream);
-  if (p.E <= 256) return launch_route_t<8, T>(p, chunks, smem, stream);
-  return launch_route_t<16, T>(p, chunks, smem, stream);
+static cudaError_t launch_route_k(const RouteParams& p, int chunks, cudaStream_t stream) {
+  if (p.top_k <= 2) return launch_route_t<2, T>(p, chunks, stream);
+  if (p.top_k <= 4) return launch_route_t<4, T>(p, chunks, stream);
+  if (p.top_k <= 6) return launch_route_t<6, T>(p, chunks, stream);
+  if (p.top_k <= 8) return launch_route_t<8, T>(p, chunks, stream);
+  if (p.top_k <= 16) return launch_route_t<16, T>(p, chunks, stream);
+  return launch_route_t<32, T>(p, chunks, stream);
 }
 
 int launch_route(const RouteArgs& a, cudaStream_t stream) {
@@ -515,6 +801,8 @@ int launch_route(const RouteArgs& a, cudaStream_t stream) {
   p.top_groups = a.top_groups;
   p.group_top = a.group_top;
   p.renorm = a.renormalize;
+  p.wide = (int64_t)a.num_experts * (a.dtype == TJ_DTYPE_F32 ? 4 : 2) % 16 == 0 &&
+           (reinterpret_cast<uintptr_t>(a.logits) & 15u) == 0;
   p.weight_scale = a.weight_scale;
   p.experts = a.experts;
   p.weights = a.weights;
@@ -522,16 +810,16 @@ int launch_route(const RouteArgs& a, cudaStream_t stream) {
   p.slot_row = a.plan + a.num_experts + 1;
   p.row_slot = p.slot_row + (int64_t)a.rows * a.top_k;
   p.hist = p.row_slot + (int64_t)a.rows * a.top_k;
-  const size_t smem = (size_t)(kRouteWarps + 2) * a.num_experts * sizeof(int);  // at most 36 KB
   cudaError_t e;
-  if (a.dtype == TJ_DTYPE_F16)
-    e = launch_route_vpl<__half>(p, chunks, smem, stream);
+  if (a.logits == nullptr)
+    e = launch_route_t<0, float>(p, chunks, stream);
+  else if (a.dtype == TJ_DTYPE_F16)
+    e = launch_route_k<__half>(p, chunks, stream);
   else if (a.dtype == TJ_DTYPE_BF16)
-    e = launch_route_vpl<__nv_bfloat16>(p, chunks, smem, stream);
+    e = launch_route_k<__nv_bfloat16>(p, chunks, stream);
   else
-    e = launch_route_vpl<float>(p, chunks, smem, stream);
-  if (e == cudaSuccess && chunks > 1)
-    e = launch_pdl(expert_plan_kernel, dim3(chunks), dim3(kRouteThreads), smem, stream, p);
+    e = launch_route_k<float>(p, chunks, stream);
+  if (e == cudaSuccess && chunks > 1) e = launch_plan(p, chunks, stream);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(TJ_ERR_CUDA, "route_experts launch: %s", cudaGetErrorString(e));
   return TJ_OK;

@@ -147,7 +147,7 @@ __device__ __forceinline__ void sandwich_stats(const float (&v)[VPL][VW], int D,
 }
 
 __device__ __forceinline__ float gate_activation(float g, int act) {
-  if (act == TJ_GATE_SIGMOID) return 1.f / (1.f + expf(-g));
+  if (act == TJ_GATE_SIGMOID) return __fdividef(1.f, 1.f + expf(-g));  // within 2 ulp; 0 where expf overflows
   if (act == TJ_GATE_TANH) return tanhf(g);
   return g;
 }
@@ -366,6 +366,14 @@ __device__ __forceinline__ void chunk_read_16(const T* row, int i, int k, int D,
     for (int e = 0; e < 4; ++e) v[e] = chunk_in<RT, false>(i, e, k, D) ? from_16(row[(4 * i + e) * RT + k]) : 0.f;
   }
 }
+// Position of column c in a per-channel vector stored chunk by chunk, so that a
+// thread's chunk is one 16-byte load either way; places past the row hold zeros.
+template <int RT, bool kVec>
+__device__ __forceinline__ int chunk_place(int c) {
+  if (kVec) return c;
+  const int n = c / RT;
+  return ((n >> 2) * RT + c % RT) * 4 + (n & 3);
+}
 __device__ __forceinline__ float2& pair(float* v, int i) { return reinterpret_cast<float2*>(v)[i]; }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
@@ -429,17 +437,21 @@ __global__ void __launch_bounds__(512, 1) sandwich_ring_kernel(const SandwichPar
     fence_barrier_init();
   }
   pdl_wait();
+  for (int i = threadIdx.x; i < (int)sh.vec_bytes; i += (int)blockDim.x)  // 4 vectors of vec_bytes / 4
+    reinterpret_cast<float*>(ring_smem)[i] = 0.f;
+  __syncthreads();
 #pragma unroll 4
   for (int c = threadIdx.x; c < D; c += (int)blockDim.x) {
+    const int at = chunk_place<RT, kVec>(c);
     float g = p.scale;
     if (sh.channel_gate) {
       const float raw = p.gate_f32 ? static_cast<const float*>(p.gate)[c] : from_16(static_cast<const T*>(p.gate)[c]);
       g *= gate_activation(raw, p.act);
     }
-    va[c] = p.post_gamma ? p.post_gamma[c] * g : g;
-    vb[c] = p.post_beta ? p.post_beta[c] * g : 0.f;
-    vg[c] = p.pre_gamma[c];
-    vh[c] = p.pre_beta ? p.pre_beta[c] : 0.f;
+    va[at] = p.post_gamma ? p.post_gamma[c] * g : g;
+    vb[at] = p.post_beta ? p.post_beta[c] * g : 0.f;
+    vg[at] = p.pre_gamma[c];
+    vh[at] = p.pre_beta ? p.pre_beta[c] : 0.f;
   }
   __syncthreads();
 
@@ -565,8 +577,13 @@ __global__ void __launch_bounds__(512, 1) sandwich_ring_kernel(const SandwichPar
     if (skip) continue;
 
     if (row_gate && p.act != TJ_GATE_NONE) {
+      if (p.act == TJ_GATE_SIGMOID) {
 #pragma unroll
-      for (int i = 0; i < 4 * C; ++i) gt[i] = gate_activation(gt[i], p.act);
+        for (int i = 0; i < 4 * C; ++i) gt[i] = gate_activation(gt[i], TJ_GATE_SIGMOID);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4 * C; ++i) gt[i] = gate_activation(gt[i], TJ_GATE_TANH);
+      }
     }
     float mean = 0.f, rstd = 1.f;
     if (p.post_gamma) team_stats<C, RT, kVec, kFull>(b, D, k, p.rms, p.eps, red, bar_id, turn, mean, rstd);
@@ -575,8 +592,8 @@ __global__ void __launch_bounds__(512, 1) sandwich_ring_kernel(const SandwichPar
 #pragma unroll
     for (int i = 0; i < C; ++i) {
       alignas(16) float a[4], c[4];
-      chunk_read<RT, kVec, kFull>(va, i, k, D, a);
-      chunk_read<RT, kVec, kFull>(vb, i, k, D, c);
+      chunk_read<RT, true, true>(va, i, k, D, a);
+      chunk_read<RT, true, true>(vb, i, k, D, c);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float2 t = fmul2(fadd2(pair(b, 2 * i + h), neg), rs);
@@ -600,8 +617,8 @@ __global__ void __launch_bounds__(512, 1) sandwich_ring_kernel(const SandwichPar
 #pragma unroll
     for (int i = 0; i < C; ++i) {
       alignas(16) float a[4], c[4];
-      chunk_read<RT, kVec, kFull>(vg, i, k, D, a);
-      chunk_read<RT, kVec, kFull>(vh, i, k, D, c);
+      chunk_read<RT, true, true>(vg, i, k, D, a);
+      chunk_read<RT, true, true>(vh, i, k, D, c);
       float2 o[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -622,26 +639,29 @@ __global__ void __launch_bounds__(512, 1) sandwich_ring_kernel(const SandwichPar
     for (int s = 0; s < sh.stages; ++s) drain_wait(bar_at(s), s < stage ? phase ^ 1 : phase);
 }
 
-// Teams and stages for the row's bytes: as many teams as fit with two stages
-// each, then as many stages (at most four).  False if not even one team fits.
-static bool ring_shape(const SandwichParams& p, int RT, bool channel_gate, int num_sms, RingShape* sh) {
+// Teams and stages for the row's bytes: two stages each while that leaves ten
+// warps to hide the sums' latency, else one (a row in flight while the team
+// computes another); then as many teams as fit and as many stages, at most
+// four.  False if not even one team fits.
+static bool ring_shape(const SandwichParams& p, int RT, int columns, bool channel_gate, int num_sms, RingShape* sh) {
   sh->slots = p.weights ? p.top_k : 1;
   sh->channel_gate = channel_gate;
-  sh->vec_bytes = ((uint32_t)p.D * 4 + 15) & ~15u;
+  sh->vec_bytes = (uint32_t)columns * 4;
   sh->x_bytes = (((uint32_t)p.D * 4 + 15) & ~15u) + 16;
   sh->b_bytes = (((uint32_t)p.D * 2 + 15) & ~15u) + 16;
   const bool row_gate = p.gate && !channel_gate;
   sh->gate_bytes = row_gate ? (((uint32_t)p.D * (p.gate_f32 ? 4 : 2) + 15) & ~15u) + 16 : 0;
   sh->stage_bytes = (uint32_t)sizeof(RingMeta) + sh->x_bytes + sh->slots * sh->b_bytes + sh->gate_bytes;
-  const uint32_t limit = 227 * 1024 - 4 * sh->vec_bytes - 1024;  // sums and barriers below 1 KB
-  if (4 * sh->vec_bytes + 1024 + 2 * (uint64_t)sh->stage_bytes > 227 * 1024) return false;
+  const int64_t limit = 227 * 1024 - 4 * (int64_t)sh->vec_bytes - 1024;  // sums and barriers below 1 KB
+  if (limit < (int64_t)sh->stage_bytes) return false;
   int teams = (int)(limit / (2 * sh->stage_bytes));
+  if (teams * RT < 10 * 32) teams = (int)(limit / sh->stage_bytes);
   const int most = 512 / RT;
   if (teams > most) teams = most;
   // no more teams than rows to give them
   const int64_t wanted = ((int64_t)p.rows + num_sms - 1) / num_sms;
   if (teams > wanted) teams = (int)wanted;
-  int stages = (int)(limit / (teams * sh->stage_bytes));
+  const int stages = (int)(limit / (teams * (int64_t)sh->stage_bytes));
   sh->teams = teams;
   sh->stages = stages > 4 ? 4 : stages;
   sh->smem = 4 * sh->vec_bytes + 1024 + (uint32_t)(teams * sh->stages) * sh->stage_bytes;
@@ -672,28 +692,29 @@ static int launch_ring_vec(const SandwichParams& p, const RingShape& sh, int num
   return launch_ring_t<C, RT, true, false, T>(p, sh, num_sms, stream);
 }
 
-// The ring takes rows of up to 4096 columns (a warp per row while a thread then
-// holds at most 32 columns of it, else 128 threads) when there are enough of
-// them to fill it; *done tells whether it did.
+// The ring takes rows of up to 4096 columns, up to 32 of them in a thread, when
+// there are enough rows to fill it; *done tells whether it did.
 template <typename T>
 static int launch_ring(const SandwichParams& p, bool wide, bool channel_gate, cudaStream_t stream, bool* done) {
   *done = false;
   int num_sms = 0;
   int rc = ensure_device_props(&num_sms);
   if (rc) return rc;
+  const int RT = p.D <= 1024 ? 32 : (p.D <= 2048 ? 64 : 128);
+  const int columns = p.D <= 256 ? 256 : (wide && p.D <= 512 ? 512 : 32 * RT);  // of the team
   RingShape sh{};
-  if (p.D > 4096 || p.rows <= 2 * num_sms || !ring_shape(p, p.D <= 1024 ? 32 : 128, channel_gate, num_sms, &sh))
-    return TJ_OK;
+  if (p.D > 4096 || p.rows <= 2 * num_sms || !ring_shape(p, RT, columns, channel_gate, num_sms, &sh)) return TJ_OK;
   *done = true;
   if (wide) {
     if (p.D <= 256) return launch_ring_vec<2, 32, T>(p, sh, num_sms, stream);
     if (p.D <= 512) return launch_ring_vec<4, 32, T>(p, sh, num_sms, stream);
     if (p.D <= 1024) return launch_ring_vec<8, 32, T>(p, sh, num_sms, stream);
-    if (p.D <= 2048) return launch_ring_vec<4, 128, T>(p, sh, num_sms, stream);
+    if (p.D <= 2048) return launch_ring_vec<8, 64, T>(p, sh, num_sms, stream);
     return launch_ring_vec<8, 128, T>(p, sh, num_sms, stream);
   }
   if (p.D <= 256) return launch_ring_t<2, 32, false, false, T>(p, sh, num_sms, stream);
   if (p.D <= 1024) return launch_ring_t<8, 32, false, false, T>(p, sh, num_sms, stream);
+  if (p.D <= 2048) return launch_ring_t<8, 64, false, false, T>(p, sh, num_sms, stream);
   return launch_ring_t<8, 128, false, false, T>(p, sh, num_sms, stream);
 }
 

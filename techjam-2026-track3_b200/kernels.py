@@ -352,6 +352,16 @@ def flash_attn_fwd(q, k, v, q_cu, kv_off, kv_len, max_q_per_sample, scale, causa
 
 
 # ---- expert feed-forward ------------------------------------------------------
+# A call on one token is bound by the host, so these wrappers make few torch
+# calls: no device guard where the device is current, the raw stream handle.
+def _launch(dev: torch.device, fn, *args) -> int:
+    """fn(*args, stream) with dev current, on dev's current stream."""
+    if torch.cuda.current_device() == dev.index:
+        return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    with torch.cuda.device(dev):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+
+
 _DTYPES = {torch.float32: _lib.TJ_DTYPE_F32, torch.float16: _lib.TJ_DTYPE_F16, torch.bfloat16: _lib.TJ_DTYPE_BF16}
 _SCORES = {"softmax": _lib.TJ_SCORE_SOFTMAX, "sigmoid": _lib.TJ_SCORE_SIGMOID}
 _GATES = {"none": _lib.TJ_GATE_NONE, "sigmoid": _lib.TJ_GATE_SIGMOID, "tanh": _lib.TJ_GATE_TANH}
@@ -464,15 +474,14 @@ def route_experts(logits, top_k, *, scoring="softmax", bias=None, num_groups=1, 
         _require_shape(bias, "bias", (E,), torch.float32, dev)
     _require_count(row_count, dev)
     lib = _lib.load()
-    with torch.cuda.device(dev):
-        experts = torch.empty(rows, top_k, dtype=torch.int32, device=dev)
-        weights = torch.empty(rows, top_k, dtype=torch.float32, device=dev)
-        plan = _plan_buffer(rows, top_k, E, dev)
-        rc = lib.tj_route_experts(
-            logits.data_ptr(), _DTYPES[logits.dtype], rows, _ptr(row_count), E, top_k, _SCORES[scoring], _ptr(bias),
-            num_groups, top_groups, group_score_top, 1 if renormalize else 0, float(weight_scale), experts.data_ptr(),
-            weights.data_ptr(), plan.data_ptr(), _stream(logits),
-        )
+    experts = torch.empty(rows, top_k, dtype=torch.int32, device=dev)
+    weights = torch.empty(rows, top_k, dtype=torch.float32, device=dev)
+    plan = _plan_buffer(rows, top_k, E, dev)
+    rc = _launch(
+        dev, lib.tj_route_experts, logits.data_ptr(), _DTYPES[logits.dtype], rows, _ptr(row_count), E, top_k,
+        _SCORES[scoring], _ptr(bias), num_groups, top_groups, group_score_top, 1 if renormalize else 0, weight_scale,
+        experts.data_ptr(), weights.data_ptr(), plan.data_ptr(),
+    )
     _lib.check(rc, "route_experts")
     return ExpertRouting(experts, weights, plan, E, row_count)
 
@@ -491,11 +500,9 @@ def expert_plan(experts, weights, num_experts, *, row_count=None) -> ExpertRouti
     _require_count(row_count, dev)
     if not 1 <= num_experts <= 512:
         raise ValueError(f"num_experts must be in 1..512, got {num_experts}")
-    lib = _lib.load()
-    with torch.cuda.device(dev):
-        plan = _plan_buffer(rows, top_k, num_experts, dev)
-        rc = lib.tj_expert_plan(experts.data_ptr(), rows, top_k, _ptr(row_count), num_experts, plan.data_ptr(),
-                                _stream(experts))
+    plan = _plan_buffer(rows, top_k, num_experts, dev)
+    rc = _launch(dev, _lib.load().tj_expert_plan, experts.data_ptr(), rows, top_k, _ptr(row_count), num_experts,
+                 plan.data_ptr())
     _lib.check(rc, "expert_plan")
     return ExpertRouting(experts, weights, plan, num_experts, row_count)
 
@@ -529,16 +536,17 @@ def gemm_experts(a, w, bias, routing, *, gather, gelu=False, out=None):
     if bias is not None:
         _require_shape(bias, "bias", (routing.num_experts, N), torch.float32, dev)
     lib = _lib.load()
-    with torch.cuda.device(dev):
-        if out is None:
-            out = torch.empty(slots, N, dtype=a.dtype, device=dev)
+    if out is None:
+        out = torch.empty(slots, N, dtype=a.dtype, device=dev)
+    else:
         _require_out(out, "out", (slots, N), a.dtype, dev)
-        need = lib.tj_gemm_experts_workspace_bytes(routing.rows, routing.top_k, routing.num_experts, K, 1 if gather else 0)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        rc = lib.tj_gemm_experts(
-            a.data_ptr(), code, 1 if gather else 0, w.data_ptr(), _ptr(bias), routing.plan.data_ptr(), routing.rows,
-            routing.top_k, routing.num_experts, N, K, 1 if gelu else 0, out.data_ptr(), _ptr(ws), need, _stream(a),
-        )
+    need = lib.tj_gemm_experts_workspace_bytes(routing.rows, routing.top_k, routing.num_experts, K, 1 if gather else 0)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    rc = _launch(
+        dev, lib.tj_gemm_experts, a.data_ptr(), code, 1 if gather else 0, w.data_ptr(), _ptr(bias),
+        routing.plan.data_ptr(), routing.rows, routing.top_k, routing.num_experts, N, K, 1 if gelu else 0,
+        out.data_ptr(), _ptr(ws), need,
+    )
     _lib.check(rc, "gemm_experts")
     return out
 
@@ -554,15 +562,14 @@ def expert_combine(y, routing, *, out=None):
         raise ValueError(f"y must be a matrix, got {tuple(y.shape)}")
     D = y.shape[1]
     _require_shape(y, "y", (routing.rows * routing.top_k, D), y.dtype, dev)
-    lib = _lib.load()
-    with torch.cuda.device(dev):
-        if out is None:
-            out = torch.empty(routing.rows, D, dtype=y.dtype, device=dev)
+    if out is None:
+        out = torch.empty(routing.rows, D, dtype=y.dtype, device=dev)
+    else:
         _require_out(out, "out", (routing.rows, D), y.dtype, dev)
-        rc = lib.tj_expert_combine(
-            y.data_ptr(), code, routing.weights.data_ptr(), routing.plan.data_ptr(), _ptr(routing.row_count),
-            routing.rows, routing.top_k, routing.num_experts, D, out.data_ptr(), _stream(y),
-        )
+    rc = _launch(
+        dev, _lib.load().tj_expert_combine, y.data_ptr(), code, routing.weights.data_ptr(), routing.plan.data_ptr(),
+        _ptr(routing.row_count), routing.rows, routing.top_k, routing.num_experts, D, out.data_ptr(),
+    )
     _lib.check(rc, "expert_combine")
     return out
 
@@ -592,17 +599,18 @@ def expert_ffn(a, w_in, b_in, w_out, b_out, routing, *, out=None):
     if b_out is not None:
         _require_shape(b_out, "b_out", (E, D), torch.float32, dev)
     lib = _lib.load()
-    with torch.cuda.device(dev):
-        if out is None:
-            out = torch.empty(routing.rows, D, dtype=a.dtype, device=dev)
-        _require_out(out, "out", (routing.rows, D), a.dtype, dev)
-        need = lib.tj_expert_ffn_workspace_bytes(routing.rows, routing.top_k, E, D, F)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        rc = lib.tj_expert_ffn(
-            a.data_ptr(), code, w_in.data_ptr(), _ptr(b_in), w_out.data_ptr(), _ptr(b_out),
-            routing.weights.data_ptr(), routing.plan.data_ptr(), _ptr(routing.row_count), routing.rows, routing.top_k,
-            E, D, F, out.data_ptr(), ws.data_ptr(), need, _stream(a),
-        )
+    rows, top_k = routing.experts.shape
+    if out is None:
+        out = torch.empty(rows, D, dtype=a.dtype, device=dev)
+    else:
+        _require_out(out, "out", (rows, D), a.dtype, dev)
+    need = lib.tj_expert_ffn_workspace_bytes(rows, top_k, E, D, F)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    rc = _launch(
+        dev, lib.tj_expert_ffn, a.data_ptr(), code, w_in.data_ptr(), _ptr(b_in), w_out.data_ptr(), _ptr(b_out),
+        routing.weights.data_ptr(), routing.plan.data_ptr(), _ptr(routing.row_count), rows, top_k, E, D, F,
+        out.data_ptr(), ws.data_ptr(), need,
+    )
     _lib.check(rc, "expert_ffn")
     return out
 
@@ -681,24 +689,23 @@ def sandwich_norm(x, branch, pre_gamma, pre_beta=None, *, post_gamma=None, post_
                 _require_shape(gate_map, "gate_map", (rows,), torch.int32, dev)
             elif gate_rows * rows_per_gate < rows:
                 raise ValueError(f"gate has {gate_rows} rows of {rows_per_gate} rows each, {rows} rows to gate")
-    lib = _lib.load()
-    with torch.cuda.device(dev):
-        if sum_out is None:
-            sum_out = torch.empty(rows, D, dtype=torch.float32, device=dev)
+    if sum_out is None:
+        sum_out = torch.empty(rows, D, dtype=torch.float32, device=dev)
+    else:
         _require_out(sum_out, "sum_out", (rows, D), torch.float32, dev)
         if row_map is not None and sum_out.data_ptr() == x.data_ptr():
             raise ValueError("sum_out cannot be x when row_map is given")
-        if out is None:
-            out = torch.empty(rows, D, dtype=branch.dtype, device=dev)
+    if out is None:
+        out = torch.empty(rows, D, dtype=branch.dtype, device=dev)
+    else:
         _require_out(out, "out", (rows, D), branch.dtype, dev)
-        desc = _lib.SandwichDesc(
-            x.data_ptr(), _ptr(row_map), branch.data_ptr(), routing.weights.data_ptr() if routing is not None else None,
-            routing.row_slot.data_ptr() if routing is not None else None, _ptr(post_gamma), _ptr(post_beta),
-            _ptr(gate), _ptr(gate_map), _ptr(pre_gamma), _ptr(pre_beta), _ptr(row_count), sum_out.data_ptr(),
-            out.data_ptr(), branch.shape[0], code, rows, x.shape[0], D, routing.top_k if routing is not None else 0,
-            gate_rows, rows_per_gate, gate_code, _GATES[gate_act], 1 if kind == "rms" else 0, float(eps),
-            float(residual_scale),
-        )
-        rc = lib.tj_sandwich_norm(ctypes.byref(desc), _stream(x))
+    desc = _lib.SandwichDesc(
+        x.data_ptr(), _ptr(row_map), branch.data_ptr(), routing.weights.data_ptr() if routing is not None else None,
+        routing.row_slot.data_ptr() if routing is not None else None, _ptr(post_gamma), _ptr(post_beta),
+        _ptr(gate), _ptr(gate_map), _ptr(pre_gamma), _ptr(pre_beta), _ptr(row_count), sum_out.data_ptr(),
+        out.data_ptr(), branch.shape[0], code, rows, x.shape[0], D, routing.top_k if routing is not None else 0,
+        gate_rows, rows_per_gate, gate_code, _GATES[gate_act], 1 if kind == "rms" else 0, eps, residual_scale,
+    )
+    rc = _launch(dev, _lib.load().tj_sandwich_norm, ctypes.byref(desc))
     _lib.check(rc, "sandwich_norm")
     return sum_out, out

@@ -43,8 +43,8 @@ def test_cpu_tensors_are_refused(pkg):
 def test_plan_and_workspace_sizes(pkg):
     lib = pkg._lib.load()
     assert lib.tj_expert_plan_ints(0, 2, 8) == 9 + 8
-    assert lib.tj_expert_plan_ints(32, 2, 8) == 9 + 128 + 8
-    assert lib.tj_expert_plan_ints(33, 2, 8) == 9 + 132 + 16
+    assert lib.tj_expert_plan_ints(64, 2, 8) == 9 + 256 + 8
+    assert lib.tj_expert_plan_ints(65, 2, 8) == 9 + 260 + 16
     assert lib.tj_expert_plan_ints(100000, 4, 64) == 65 + 800000 + 148 * 64
     assert lib.tj_expert_plan_ints(-1, 2, 8) == 0 and lib.tj_expert_plan_ints(1, 0, 8) == 0
     assert lib.tj_expert_ffn_workspace_bytes(10, 2, 4, 64, 128) == 20 * 256 + 20 * 256
