@@ -545,6 +545,7 @@ int tj_expert_ffn(const void* a, int dtype, const void* w_in, const float* b_in,
   g.gather = 0;
   g.gelu = 0;
   g.out_f32 = 1;
+  g.plan_ready = 1;
   g.a_rows = slots;
   g.N = d_model;
   g.K = ffn_dim;

@@ -67,6 +67,11 @@ struct XpParams {
   const float* bias;        // [E][N] or null
   void* out;                // [slots][N]
   int slots, rows, E, N, K;
+  // 1: the plan and the weights were there before the preceding kernel of the
+  // stream started (tj_expert_ffn's FFN-out: FFN-in has waited for the router),
+  // so only what reads or writes activations waits for that kernel, and an SM
+  // that is done with it loads weights while the others finish.
+  int plan_ready;
   int splits;               // parts of K; part i writes plane i of out [splits][slots][N]
 };
 
@@ -240,7 +245,7 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
       tmem_relinquish();
     }
   }
-  pdl_wait();
+  if (!p.plan_ready) pdl_wait();
   const int m_tiles = (p.N + Cfg::kFeatures - 1) / Cfg::kFeatures;
   // Offsets, held inside [0, slots] whatever the plan says.
   for (int e = threadIdx.x; e <= p.E; e += kXpThreads) {
@@ -301,6 +306,7 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
           if (last_parity[s] >= 0) drain_wait(full_bar(s), (uint32_t)last_parity[s]);
     }
   } else if (warp == 1) {
+    if (p.plan_ready) pdl_wait();
     Walk walk(first, tiles, p.E, m_tiles, p.splits, tile_step);
     int stage = 0;
     uint32_t phase = 0;
@@ -408,6 +414,7 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
       }
     }
   } else if (warp >= 4) {
+    if (p.plan_ready) pdl_wait();
     Walk walk(first, tiles, p.E, m_tiles, p.splits, tile_step);
     const int quarter = warp & 3;
     const int group = (warp - 4) >> 2;
@@ -695,15 +702,18 @@ static int launch_expert_gather(const ExpertGemmArgs& a, void* out, cudaStream_t
 // 32 on average, else one CTA with tiles of up to 32.
 static bool experts_gemm_pairs(int64_t slots, int num_experts) { return slots > 32 * (int64_t)num_experts; }
 
-// Parts of K for the fp32 planes: while the experts have few rows and the
-// tiles (each of the experts that can be reached, 128 features) do not give
-// every SM about four, and a part keeps four K steps of 64.
+// Parts of K for the fp32 planes while the experts have few rows: as many as
+// still fit one wave of CTAs with the tiles (128 features of each expert that
+// can be reached), four K steps of 64 to a part at least.  One token, two experts,
+// K 4096: 8 parts, 19.8 us for the whole FFN instead of 25.5 with 16; above a
+// wave splitting only adds planes (33 tokens, 64 experts: 84.5 us unsplit, 87
+// and 90 us in two and four parts).
 int experts_gemm_splits(int64_t slots, int num_experts, int n, int k) {
   if (experts_gemm_pairs(slots, num_experts)) return 1;
   const int64_t tiles = (slots < num_experts ? slots : num_experts) * ((n + kBM - 1) / kBM);
   const int k_blocks = (k + kBK - 1) / kBK;
   int splits = 1;
-  while (2 * splits * 4 <= k_blocks && tiles * splits < 4 * 148) splits *= 2;
+  while (2 * splits * 4 <= k_blocks && 2 * splits * tiles <= 148) splits *= 2;
   const int part = (k_blocks + splits - 1) / splits;
   return (k_blocks + part - 1) / part;  // none of them empty
 }
@@ -739,6 +749,7 @@ int launch_experts_gemm(const ExpertGemmArgs& a, cudaStream_t stream) {
   kp.E = a.num_experts;
   kp.N = a.N;
   kp.K = a.K;
+  kp.plan_ready = a.plan_ready;
   kp.splits = a.out_f32 ? experts_gemm_splits(a.slots, a.num_experts, a.N, a.K) : 1;
   if (experts_gemm_pairs(a.slots, a.num_experts)) {
     ExpertGemmArgs g = a;

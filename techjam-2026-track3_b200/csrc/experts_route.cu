@@ -322,6 +322,9 @@ __device__ void route_choose(const RouteParams& p, const float* bias, float bias
       }
     }
     for (int o = L >> 1; o > 0; o >>= 1) kept |= __shfl_xor_sync(0xffffffffu, kept, o);
+    // Threads past the tile's rows follow along on row 0, whose strengths another
+    // warp may be writing: they keep no group.
+    if (!on) kept = 0;
     weakest = -row_max(-weakest, L);
     dropped = row_max(dropped, L);
     // a strength is a rounded sum of up to two values
@@ -331,7 +334,7 @@ __device__ void route_choose(const RouteParams& p, const float* bias, float bias
   list.clear();
   if (p.groups > 1) {
     // only the groups kept, each row its own, in index order
-    for (int i = 0; i < p.top_groups; ++i) {
+    while (kept != 0) {
       const int g = __ffs(kept) - 1;
       kept &= kept - 1;
       const int e0 = g * per;
@@ -523,7 +526,7 @@ __global__ void __launch_bounds__(KL > 16 ? 512 : kRouteThreads) route_kernel(co
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool alone = gridDim.x == 1;
   for (int i = threadIdx.x; i < p.E; i += (int)blockDim.x) hist[i] = 0;
-  if (alone) pdl_trigger();  // the other SMs set up what follows meanwhile
+  pdl_trigger();  // what follows sets up meanwhile, where there is room
   pdl_wait();
   const int live = p.row_count ? max(0, min(p.rows, *p.row_count)) : p.rows;
   const int r0 = (int)min((int64_t)blockIdx.x * p.chunk_rows, (int64_t)p.rows);
@@ -622,7 +625,6 @@ __global__ void __launch_bounds__(KL > 16 ? 512 : kRouteThreads) route_kernel(co
   }
   __syncthreads();
   if (!alone) {
-    pdl_trigger();
     for (int i = threadIdx.x; i < p.E; i += (int)blockDim.x) p.hist[(int64_t)blockIdx.x * p.E + i] = hist[i];
     return;
   }
@@ -646,6 +648,7 @@ __global__ void __launch_bounds__(kRouteThreads) expert_plan_kernel(const RouteP
   __shared__ int used;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int i = threadIdx.x; i < 2 * p.E; i += kRouteThreads) route_smem[i] = 0;
+  pdl_trigger();
   __syncthreads();
   pdl_wait();
   // Thread group q of E consecutive threads sums chunks q, q + groups, ...

@@ -164,6 +164,7 @@ struct ExpertGemmArgs {
   const int32_t* slot_row;  // [slots]
   int dtype, gather, gelu;
   int out_f32;              // out: float [experts_gemm_splits][slots][N] (not with gather or gelu)
+  int plan_ready;           // the plan and w precede the preceding kernel of the stream
   int slots, a_rows, num_experts, N, K;
   void* out;                // [slots][N]
   void* workspace;          // gather: experts_gemm_workspace bytes

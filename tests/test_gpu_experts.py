@@ -143,6 +143,18 @@ def test_route_groups_and_bias(cuda_pkg, rows, E, k, groups, top, scoring, biase
         _check_route(cuda_pkg, logits, k, scoring, bias=bias, groups=groups, top_groups=top, group_top=group_top)
 
 
+# Tiles whose last rows do not fill their warps, in every chunk but one.
+@pytest.mark.parametrize("rows", [9473, 90077])
+def test_route_groups_partial_tiles(cuda_pkg, rows):
+    g = _gen(rows)
+    logits = _randn(g, rows, 64, std=1.5)
+    logits[torch.rand(rows, generator=g, device=DEV) < 0.02] = -math.inf
+    bias = _randn(g, 64, std=0.05)
+    for _ in range(3):
+        _check_route(cuda_pkg, logits, 6, "sigmoid", bias=bias, groups=8, top_groups=3, group_top=2, scale=2.5)
+    _check_route(cuda_pkg, logits, 4, "softmax", groups=4, top_groups=1)
+
+
 @pytest.mark.parametrize("E,groups,top", [(64, 1, 1), (200, 1, 1), (64, 8, 3)])
 def test_route_values_closer_than_fp32(cuda_pkg, E, groups, top):
     """The bias nearly cancels the score: all values lie within 1e-7 and only
