@@ -16,9 +16,8 @@
 //
 // Plan: a stable counting sort of the (row, j) pairs by expert, in (row, j)
 // order inside an expert.  Each CTA of the router owns a chunk of rows and
-// writes its histogram; a second kernel (one CTA per chunk) sums the
-// histograms of the chunks before it and ranks its own pairs with warp
-// matches.  No atomic decides an order, so the plan is the same on every run.
+// writes its histogram; a second kernel (one CTA per chunk) adds up the
+// histograms of the chunks before it and ranks its own pairs with warp matches.  No atomic decides an order, so the plan is the same on every run.
 // Up to kRouteRowsPerCta rows fit one CTA, which then does both.
 // The router reads rows * E logits and writes 16 bytes per pair.
 //
@@ -38,7 +37,8 @@
 namespace tj {
 
 constexpr int kRouteThreads = 1024;
-constexpr int kRouteWarps = kRouteThreads / 32;
+constexpr int kSortThreads = 1024;
+constexpr int kMaybe = 16;       // candidates a lane notes before it sorts them in
 constexpr int kPlanTile = 4096;  // pairs sorted at a time
 constexpr int kRouteRowsPerCta = 64;
 constexpr int kRouteMaxChunks = 148;  // one CTA per SM; also the rows of the histogram table
@@ -246,8 +246,8 @@ struct RouteList {
 // top[row], zs[row] for the weights.  All threads of a warp take part.
 template <int KL, typename T>
 __device__ void route_choose(const RouteParams& p, const float* bias, float bias_max, float* xs, int pitch,
-                             const int* flags, float* strengths, float* tops, float* zs, uint16_t* chosen, int t0,
-                             int n, int L) {
+                             const int* flags, float* strengths, float* tops, float* zs, uint16_t* maybe,
+                             uint16_t* chosen, int t0, int n, int L) {
   const int row = (int)threadIdx.x / L, sub = (int)threadIdx.x & (L - 1), lane = (int)threadIdx.x & 31;
   const bool on = row < n;
   const int E = p.E;
@@ -342,8 +342,36 @@ __device__ void route_choose(const RouteParams& p, const float* bias, float bias
       for (int e = e0 + ((sub - e0) & (L - 1)); e < e0 + per; e += L) list.push(x[e * pitch], e);
     }
   } else {
+    // With many experts to a lane: two greatest of each lane make 2 L values, so
+    // the least of the lanes' second values bounds the greatest top_k + 1 from
+    // below, and only the few experts above it are sorted in.
+    if (2 * L > p.top_k && E >= 16 * L) {
+      float a = neg_inf<float>(), b = neg_inf<float>();
+#pragma unroll 4
+      for (int e = sub; e < E; e += L) push_top2(a, b, value(e));
+      const float least = -row_max(-b, L);
+      int n = 0;
+      uint16_t* some = maybe + threadIdx.x;
+#pragma unroll 4
+      for (int e = sub; e < E; e += L) {
+        const float v = x[e * pitch];
+        if (v >= least && v > neg_inf<float>()) {
+          if (n < kMaybe) some[n * (int)blockDim.x] = (uint16_t)e;
+          ++n;
+        }
+      }
+      if (n <= kMaybe) {
+        for (int i = 0; i < n; ++i) {
+          const int e = some[i * (int)blockDim.x];
+          list.push(x[e * pitch], e);
+        }
+      } else {  // many equal values
+        for (int e = sub; e < E; e += L) list.push(x[e * pitch], e);
+      }
+    } else {
 #pragma unroll 2
-    for (int e = sub; e < E; e += L) list.push(value(e), e);
+      for (int e = sub; e < E; e += L) list.push(value(e), e);
+    }
   }
   // Merge: the best head of the lanes' lists, top_k times.
   float before = -neg_inf<float>();
@@ -439,8 +467,8 @@ __device__ void route_weights(const RouteParams& p, const int* flags, const floa
 
 // Shared memory of the sort, after `vectors` arrays of E ints.
 __device__ __forceinline__ int* plan_runs(int* smem, int vectors, int E) { return smem + vectors * E; }
-__device__ __forceinline__ uint16_t* plan_tile(int* smem, int vectors, int E) {
-  return reinterpret_cast<uint16_t*>(smem + (vectors + ((int)blockDim.x >> 5)) * E);
+__device__ __forceinline__ uint16_t* plan_tile(int* smem, int vectors, int warps, int E) {
+  return reinterpret_cast<uint16_t*>(smem + (vectors + warps) * E);
 }
 static size_t plan_smem(int vectors, int warps, int E) {
   return (size_t)(vectors + warps) * E * sizeof(int) + kPlanTile * sizeof(uint16_t);
@@ -479,11 +507,15 @@ __device__ void plan_sort(const RouteParams& p, int i0, int n, const uint16_t* t
   __syncthreads();
   for (int e = threadIdx.x; e < p.E; e += (int)blockDim.x) {
     int at = base[e];
-#pragma unroll 8
-    for (int w = 0; w < warps; ++w) {
-      const int c = runs[w * p.E + e];
-      runs[w * p.E + e] = at;
-      at += c;
+    for (int w0 = 0; w0 < warps; w0 += 8) {
+      int c[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c[i] = w0 + i < warps ? runs[(w0 + i) * p.E + e] : 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (w0 + i < warps) runs[(w0 + i) * p.E + e] = at;
+        at += c[i];
+      }
     }
     base[e] = at;
   }
@@ -514,17 +546,17 @@ __device__ void plan_fill_unused(const RouteParams& p, int used) {
 
 // Router over one chunk of rows per CTA (or, without logits, a check of the
 // given choices) and the chunk's histogram; with one chunk, the plan too.
-// Dynamic shared memory: plan_smem(2, warps, E), then the tile: logits and
-// strengths [(E + groups) * pitch], flags, tops and zs [tile_rows].  KL: 0
+// Dynamic shared memory: plan_smem(2, alone ? warps : 0, E), then the tile: logits and
+// strengths [(E + groups) * pitch], flags, tops and zs [tile_rows], candidates.  KL: 0
 // without logits.
 template <int KL, typename T>
 __global__ void __launch_bounds__(KL > 16 ? 512 : kRouteThreads) route_kernel(const RouteParams p) {
   extern __shared__ int route_smem[];
   int* hist = route_smem;                                      // [E]
   float* bias = reinterpret_cast<float*>(route_smem + p.E);    // [E]
-  uint16_t* tile = plan_tile(route_smem, 2, p.E);              // choices: of the chunk if it is the only one
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool alone = gridDim.x == 1;
+  uint16_t* tile = plan_tile(route_smem, 2, alone ? (int)blockDim.x >> 5 : 0, p.E);  // choices: of the chunk if alone
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int i = threadIdx.x; i < p.E; i += (int)blockDim.x) hist[i] = 0;
   pdl_trigger();  // what follows sets up meanwhile, where there is room
   pdl_wait();
@@ -537,6 +569,7 @@ __global__ void __launch_bounds__(KL > 16 ? 512 : kRouteThreads) route_kernel(co
     int* flags = reinterpret_cast<int*>(strengths + (p.groups > 1 ? p.groups * p.pitch : 0));
     float* tops = reinterpret_cast<float*>(flags + p.tile_rows);
     float* zs = tops + p.tile_rows;
+    uint16_t* maybe = reinterpret_cast<uint16_t*>(zs + p.tile_rows);  // [kMaybe][threads], with 16 experts a lane
     float bias_max = 0.f;
     if (p.bias) {
       for (int i = threadIdx.x; i < p.E; i += (int)blockDim.x) {
@@ -605,7 +638,7 @@ __global__ void __launch_bounds__(KL > 16 ? 512 : kRouteThreads) route_kernel(co
       else
         stage(std::integral_constant<int, 1>());
       __syncthreads();
-      route_choose<KL, T>(p, bias, bias_max, xs, p.pitch, flags, strengths, tops, zs, chosen, t0, n, p.lanes);
+      route_choose<KL, T>(p, bias, bias_max, xs, p.pitch, flags, strengths, tops, zs, maybe, chosen, t0, n, p.lanes);
       route_weights<T>(p, flags, tops, zs, chosen, t0, n, live, p.lanes);
       __syncthreads();
       for (int i = threadIdx.x; i < n * p.top_k; i += (int)blockDim.x)
@@ -640,27 +673,37 @@ __global__ void __launch_bounds__(KL > 16 ? 512 : kRouteThreads) route_kernel(co
 }
 
 // Plan of several chunks.  Dynamic shared memory: plan_smem(2, warps, E).
-__global__ void __launch_bounds__(kRouteThreads) expert_plan_kernel(const RouteParams p) {
+__global__ void __launch_bounds__(kSortThreads) expert_plan_kernel(const RouteParams p) {
   extern __shared__ int route_smem[];
   int* total = route_smem;           // [E], then its exclusive scan
   int* base = route_smem + p.E;      // [E] pairs of the chunks before this one
-  uint16_t* tile = plan_tile(route_smem, 2, p.E);
+  uint16_t* tile = plan_tile(route_smem, 2, kSortThreads / 32, p.E);
   __shared__ int used;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int i = threadIdx.x; i < 2 * p.E; i += kRouteThreads) route_smem[i] = 0;
+  for (int i = threadIdx.x; i < 2 * p.E; i += kSortThreads) route_smem[i] = 0;
   pdl_trigger();
   __syncthreads();
   pdl_wait();
-  // Thread group q of E consecutive threads sums chunks q, q + groups, ...
-  const int groups = kRouteThreads / p.E;
+  // Thread group q of E consecutive threads sums chunks q, q + groups, ..., with
+  // kFlight loads in flight (one after the other each costs a trip to the other
+  // die's L2: 17 us instead of 12 for the plan of 16384 rows of 256 experts).
+  const int groups = kSortThreads / p.E;
   if ((int)threadIdx.x < p.E * groups) {
     const int ex = (int)threadIdx.x % p.E, q = (int)threadIdx.x / p.E;
+    constexpr int kFlight = 20;
     int all = 0, before = 0;
-#pragma unroll 8
-    for (int c = q; c < (int)gridDim.x; c += groups) {
-      const int n = __ldcg(p.hist + (int64_t)c * p.E + ex);
-      all += n;
-      before += c < (int)blockIdx.x ? n : 0;
+    for (int c0 = q; c0 < (int)gridDim.x; c0 += kFlight * groups) {
+      int n[kFlight];
+#pragma unroll
+      for (int i = 0; i < kFlight; ++i) {
+        const int c = c0 + i * groups;
+        n[i] = c < (int)gridDim.x ? __ldcg(p.hist + (int64_t)c * p.E + ex) : 0;
+      }
+#pragma unroll
+      for (int i = 0; i < kFlight; ++i) {
+        all += n[i];
+        before += c0 + i * groups < (int)blockIdx.x ? n[i] : 0;
+      }
     }
     atomicAdd(total + ex, all);
     atomicAdd(base + ex, before);
@@ -672,8 +715,8 @@ __global__ void __launch_bounds__(kRouteThreads) expert_plan_kernel(const RouteP
   }
   __syncthreads();
   if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i <= p.E; i += kRouteThreads) p.offsets[i] = i < p.E ? total[i] : used;
-  for (int i = threadIdx.x; i < p.E; i += kRouteThreads) base[i] += total[i];
+    for (int i = threadIdx.x; i <= p.E; i += kSortThreads) p.offsets[i] = i < p.E ? total[i] : used;
+  for (int i = threadIdx.x; i < p.E; i += kSortThreads) base[i] += total[i];
   plan_fill_unused(p, used);
   const int live = p.row_count ? max(0, min(p.rows, *p.row_count)) : p.rows;
   const int r0 = (int)min((int64_t)blockIdx.x * p.chunk_rows, (int64_t)p.rows);
@@ -682,8 +725,8 @@ __global__ void __launch_bounds__(kRouteThreads) expert_plan_kernel(const RouteP
   for (int b = i0; b < i1; b += kPlanTile) {
     const int n = min(kPlanTile, i1 - b);
 #pragma unroll
-    for (int u = 0; u < kPlanTile / kRouteThreads; ++u) {
-      const int i = u * kRouteThreads + (int)threadIdx.x;
+    for (int u = 0; u < kPlanTile / kSortThreads; ++u) {
+      const int i = u * kSortThreads + (int)threadIdx.x;
       if (i < n) {
         const int e = b + i < on ? p.experts[b + i] : -1;
         tile[i] = e >= 0 && e < p.E ? (uint16_t)e : kNoChoice;
@@ -699,8 +742,8 @@ constexpr size_t kRouteMaxSmem = 226 * 1024;  // with the static part, below 227
 // Rows of a tile and lanes of a row: as many rows of the chunk as fit (with the
 // sort's part of shared memory, and the tile's choices in kPlanTile places),
 // in equal tiles, then as many lanes as the threads allow and the experts need.
-static void route_tile(RouteParams* p, int max_threads) {
-  const size_t fixed = plan_smem(2, kRouteWarps, p->E) + 64;
+static void route_tile(RouteParams* p, int max_threads, bool alone) {
+  const size_t fixed = plan_smem(2, alone ? kRouteThreads / 32 : 0, p->E) + 64 + (size_t)kMaybe * max_threads * 2;
   const size_t per_row = (size_t)(p->E + (p->groups > 1 ? p->groups : 0)) * 4 + 12;
   int64_t rows = (int64_t)((kRouteMaxSmem - fixed) / per_row) - 2;  // - 2: the pitch is odd
   rows = min(rows, (int64_t)max_threads);
@@ -720,14 +763,15 @@ static cudaError_t launch_route_t(RouteParams p, int chunks, cudaStream_t stream
   int threads = kMost;
   size_t tile_bytes = 0;
   if (KL > 0) {
-    route_tile(&p, kMost);
+    route_tile(&p, kMost, chunks == 1);
     threads = (p.tile_rows * p.lanes + 31) / 32 * 32;
     if (threads < 128) threads = 128;
-    tile_bytes = ((size_t)(p.E + (p.groups > 1 ? p.groups : 0)) * p.pitch + 3 * (size_t)p.tile_rows) * 4;
+    tile_bytes = ((size_t)(p.E + (p.groups > 1 ? p.groups : 0)) * p.pitch + 3 * (size_t)p.tile_rows) * 4 +
+                 (size_t)kMaybe * threads * 2;
   } else if (chunks == 1) {
     threads = p.rows * p.top_k <= 256 ? 128 : kMost;
   }
-  const size_t smem = plan_smem(2, threads / 32, p.E) + tile_bytes;
+  const size_t smem = plan_smem(2, chunks == 1 ? threads / 32 : 0, p.E) + tile_bytes;
   static bool attr_set[64] = {};
   const int dev = device_index();
   if (!attr_set[dev]) {
@@ -744,11 +788,11 @@ static cudaError_t launch_plan(const RouteParams& p, int chunks, cudaStream_t st
   const int dev = device_index();
   if (!attr_set[dev]) {
     cudaError_t e = cudaFuncSetAttribute(expert_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)plan_smem(2, kRouteWarps, kRouteMaxExperts));
+                                         (int)plan_smem(2, kSortThreads / 32, kRouteMaxExperts));
     if (e != cudaSuccess) return e;
     attr_set[dev] = true;
   }
-  return launch_pdl(expert_plan_kernel, dim3(chunks), dim3(kRouteThreads), plan_smem(2, kRouteWarps, p.E), stream, p);
+  return launch_pdl(expert_plan_kernel, dim3(chunks), dim3(kSortThreads), plan_smem(2, kSortThreads / 32, p.E), stream, p);
 }
 
 template <typename T>
