@@ -369,8 +369,10 @@ _GATES = {"none": _lib.TJ_GATE_NONE, "sigmoid": _lib.TJ_GATE_SIGMOID, "tanh": _l
 
 def _no_grad(*tensors) -> None:
     """Forward only, like the encoder: a call whose gradient would be lost raises."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("autograd through this operator is not supported; call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("autograd through this operator is not supported; call it under torch.no_grad()")
 
 
 def _cuda_tensor(t, name: str) -> torch.device:
@@ -382,9 +384,10 @@ def _cuda_tensor(t, name: str) -> torch.device:
 
 
 def _require_shape(t, name: str, shape, dtype: torch.dtype, device: torch.device) -> None:
+    if isinstance(t, torch.Tensor) and t.shape == shape and t.dtype == dtype and t.device == device and t.is_contiguous():
+        return
     _require(t, name, dtype, device)
-    if tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
 def _require_count(row_count, device: torch.device) -> None:
@@ -392,6 +395,14 @@ def _require_count(row_count, device: torch.device) -> None:
         _require(row_count, "row_count", torch.int32, device)
         if row_count.numel() != 1:
             raise ValueError("row_count must hold one int32")
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two contiguous tensors share bytes."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    return (a.data_ptr() < b.data_ptr() + b.numel() * b.element_size()
+            and b.data_ptr() < a.data_ptr() + a.numel() * a.element_size())
 
 
 def _half_dtype(t: torch.Tensor, name: str) -> int:
@@ -413,6 +424,26 @@ class ExpertRouting:
     plan: torch.Tensor
     num_experts: int
     row_count: Optional[torch.Tensor] = None
+
+    def __post_init__(self) -> None:
+        # the kernels take these buffers by pointer
+        if self.experts.dim() != 2:
+            raise ValueError(f"experts must be [rows, top_k], got {tuple(self.experts.shape)}")
+        dev = self.plan.device
+        _require(self.experts, "experts", torch.int32, dev)
+        _require_shape(self.weights, "weights", self.experts.shape, torch.float32, dev)
+        _require(self.plan, "plan", torch.int32, dev)
+        if self.plan.numel() < self.num_experts + 1 + 2 * self.experts.numel():
+            raise ValueError(f"plan of {self.plan.numel()} entries is too short for {tuple(self.experts.shape)} choices "
+                             f"of {self.num_experts} experts")
+        _require_count(self.row_count, dev)
+
+    @classmethod
+    def _made(cls, experts, weights, plan, num_experts, row_count) -> "ExpertRouting":
+        """From buffers made here, without the checks."""
+        r = cls.__new__(cls)
+        r.experts, r.weights, r.plan, r.num_experts, r.row_count = experts, weights, plan, num_experts, row_count
+        return r
 
     @property
     def rows(self) -> int:
@@ -483,7 +514,7 @@ def route_experts(logits, top_k, *, scoring="softmax", bias=None, num_groups=1, 
         experts.data_ptr(), weights.data_ptr(), plan.data_ptr(),
     )
     _lib.check(rc, "route_experts")
-    return ExpertRouting(experts, weights, plan, E, row_count)
+    return ExpertRouting._made(experts, weights, plan, E, row_count)
 
 
 def expert_plan(experts, weights, num_experts, *, row_count=None) -> ExpertRouting:
@@ -504,7 +535,7 @@ def expert_plan(experts, weights, num_experts, *, row_count=None) -> ExpertRouti
     rc = _launch(dev, _lib.load().tj_expert_plan, experts.data_ptr(), rows, top_k, _ptr(row_count), num_experts,
                  plan.data_ptr())
     _lib.check(rc, "expert_plan")
-    return ExpertRouting(experts, weights, plan, num_experts, row_count)
+    return ExpertRouting._made(experts, weights, plan, num_experts, row_count)
 
 
 def _require_routing(routing, device: torch.device) -> None:
@@ -535,11 +566,13 @@ def gemm_experts(a, w, bias, routing, *, gather, gelu=False, out=None):
     N = w.shape[1]
     if bias is not None:
         _require_shape(bias, "bias", (routing.num_experts, N), torch.float32, dev)
-    lib = _lib.load()
     if out is None:
         out = torch.empty(slots, N, dtype=a.dtype, device=dev)
     else:
         _require_out(out, "out", (slots, N), a.dtype, dev)
+        if _overlap(out, a) or _overlap(out, w):
+            raise ValueError("out must not share memory with a or w")
+    lib = _lib.load()
     need = lib.tj_gemm_experts_workspace_bytes(routing.rows, routing.top_k, routing.num_experts, K, 1 if gather else 0)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     rc = _launch(
@@ -566,6 +599,8 @@ def expert_combine(y, routing, *, out=None):
         out = torch.empty(routing.rows, D, dtype=y.dtype, device=dev)
     else:
         _require_out(out, "out", (routing.rows, D), y.dtype, dev)
+        if _overlap(out, y):
+            raise ValueError("out must not share memory with y")
     rc = _launch(
         dev, _lib.load().tj_expert_combine, y.data_ptr(), code, routing.weights.data_ptr(), routing.plan.data_ptr(),
         _ptr(routing.row_count), routing.rows, routing.top_k, routing.num_experts, D, out.data_ptr(),
@@ -632,7 +667,8 @@ def sandwich_norm(x, branch, pre_gamma, pre_beta=None, *, post_gamma=None, post_
     row r reading gate row gate_map[r] // rows_per_gate (gate_map: int32,
     default row_map, else r): a sample's gate with rows_per_gate = seq_len, a
     token's with 1.  act: none, sigmoid or tanh.  x [x_rows, D] float32; sum_out
-    may be x when there is no row_map.  Rows at or past row_count (default:
+    may be x when there is no row_map, out branch when there is no routing.  Rows
+    at or past row_count (default:
     the routing's) are left as they were."""
     dev = _cuda_tensor(x, "x")
     _no_grad(x, branch, pre_gamma, pre_beta, post_gamma, post_beta, gate)
@@ -654,6 +690,8 @@ def sandwich_norm(x, branch, pre_gamma, pre_beta=None, *, post_gamma=None, post_
         if row_count is None:
             row_count = routing.row_count
     else:
+        if branch.dim() != 2:
+            raise ValueError(f"branch must be [rows, {D}], got {tuple(branch.shape)}")
         rows = branch.shape[0]
         _require_shape(branch, "branch", (rows, D), branch.dtype, dev)
     _require_count(row_count, dev)
@@ -661,12 +699,16 @@ def sandwich_norm(x, branch, pre_gamma, pre_beta=None, *, post_gamma=None, post_
         _require_shape(row_map, "row_map", (rows,), torch.int32, dev)
     elif x.shape[0] < rows:
         raise ValueError(f"x must have at least {rows} rows, got {x.shape[0]}")
-    for name, t in (("pre_gamma", pre_gamma), ("pre_beta", pre_beta), ("post_gamma", post_gamma),
-                    ("post_beta", post_beta)):
-        if t is not None:
-            _require_shape(t, name, (D,), torch.float32, dev)
+    vector = (D,)
     if pre_gamma is None:
         raise ValueError("pre_gamma is required")
+    _require_shape(pre_gamma, "pre_gamma", vector, torch.float32, dev)
+    if pre_beta is not None:
+        _require_shape(pre_beta, "pre_beta", vector, torch.float32, dev)
+    if post_gamma is not None:
+        _require_shape(post_gamma, "post_gamma", vector, torch.float32, dev)
+    if post_beta is not None:
+        _require_shape(post_beta, "post_beta", vector, torch.float32, dev)
     if post_beta is not None and post_gamma is None:
         raise ValueError("post_beta needs post_gamma")
     gate_rows, gate_code = 0, _lib.TJ_DTYPE_F32
@@ -693,12 +735,18 @@ def sandwich_norm(x, branch, pre_gamma, pre_beta=None, *, post_gamma=None, post_
         sum_out = torch.empty(rows, D, dtype=torch.float32, device=dev)
     else:
         _require_out(sum_out, "sum_out", (rows, D), torch.float32, dev)
-        if row_map is not None and sum_out.data_ptr() == x.data_ptr():
-            raise ValueError("sum_out cannot be x when row_map is given")
+        if _overlap(sum_out, x) and (row_map is not None or sum_out.data_ptr() != x.data_ptr()):
+            raise ValueError("sum_out may share memory with x only as x itself, without row_map")
+        if _overlap(sum_out, branch):
+            raise ValueError("sum_out must not share memory with branch")
     if out is None:
         out = torch.empty(rows, D, dtype=branch.dtype, device=dev)
     else:
         _require_out(out, "out", (rows, D), branch.dtype, dev)
+        if _overlap(out, branch) and (routing is not None or out.data_ptr() != branch.data_ptr()):
+            raise ValueError("out may share memory with branch only as branch itself, without routing")
+        if _overlap(out, x) or _overlap(out, sum_out):
+            raise ValueError("out must not share memory with x or sum_out")
     desc = _lib.SandwichDesc(
         x.data_ptr(), _ptr(row_map), branch.data_ptr(), routing.weights.data_ptr() if routing is not None else None,
         routing.row_slot.data_ptr() if routing is not None else None, _ptr(post_gamma), _ptr(post_beta),

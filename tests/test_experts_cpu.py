@@ -174,3 +174,34 @@ def test_sandwich_refusals(k, kw, error):
     args.update(kw)
     with pytest.raises(error):
         k.sandwich_norm(**args)
+
+
+def test_outputs_that_share_memory_are_refused(k):
+    r = _routing(k, rows=4, top_k=1)
+    a = torch.zeros(4, 16, dtype=F16)
+    with pytest.raises(ValueError, match="share"):
+        k.gemm_experts(a, torch.zeros(3, 16, 16, dtype=F16), None, r, gather=False, out=a)
+    with pytest.raises(ValueError, match="share"):
+        k.expert_combine(a, r, out=a)
+    big = torch.zeros(5, 16)
+    x, gamma = big[:4], torch.ones(16)
+    with pytest.raises(_Unreached):
+        k.sandwich_norm(x, a, gamma, sum_out=x, out=a)
+    for kw in (dict(sum_out=big[1:]), dict(sum_out=x, row_map=torch.zeros(4, dtype=I32)), dict(out=a, routing=r)):
+        with pytest.raises(ValueError, match="share"):
+            k.sandwich_norm(x, a, gamma, **kw)
+    half = torch.zeros(4, 32, dtype=F16)
+    with pytest.raises(ValueError, match="share"):
+        k.sandwich_norm(half.view(torch.float32), a, gamma, out=half.view(8, 16)[:4])
+
+
+@pytest.mark.parametrize("experts,weights,plan,error", [
+    (torch.zeros(4, 2, dtype=I32), torch.zeros(4, 1), torch.zeros(20, dtype=I32), ValueError),
+    (torch.zeros(4, 2), torch.zeros(4, 2), torch.zeros(20, dtype=I32), TypeError),
+    (torch.zeros(4, 2, dtype=I32), torch.zeros(4, 2), torch.zeros(19, dtype=I32), ValueError),
+    (torch.zeros(8, dtype=I32), torch.zeros(8), torch.zeros(20, dtype=I32), ValueError),
+])
+def test_routing_buffers_are_checked(k, experts, weights, plan, error):
+    k.ExpertRouting(torch.zeros(4, 2, dtype=I32), torch.zeros(4, 2), torch.zeros(20, dtype=I32), 3)
+    with pytest.raises(error):
+        k.ExpertRouting(experts, weights, plan, 3)

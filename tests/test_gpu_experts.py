@@ -210,6 +210,46 @@ def test_route_far_logits(cuda_pkg):
     _check_route(cuda_pkg, logits + 400.0, 4, "sigmoid", renorm=False)
 
 
+def test_route_past_32_bit_offsets(cuda_pkg):
+    """rows * experts above 2^31 elements."""
+    rows, E = 8_400_000, 256
+    logits = torch.empty(rows, E, device=DEV, dtype=torch.bfloat16)
+    g = _gen(21)
+    for c in logits.split(600_000):
+        c.normal_(generator=g)
+    r = cuda_pkg.kernels.route_experts(logits, 1, renormalize=False, scoring="sigmoid")
+    e = torch.arange(E, device=DEV, dtype=torch.int32)
+    for lo in range(0, rows, 600_000):
+        c = logits[lo : lo + 600_000]
+        first = torch.where(c == c.amax(1, keepdim=True), e, E).amin(1)
+        assert torch.equal(r.experts[lo : lo + 600_000, 0], first)
+    flat = r.experts.flatten().long()
+    assert torch.equal(r.offsets[1:].long(), torch.bincount(flat, minlength=E).cumsum(0))
+    assert torch.equal(r.slot_row.long(), flat.sort(stable=True)[1])
+
+
+@pytest.mark.parametrize("kw", [dict(num_groups=3), dict(num_groups=0), dict(num_groups=64, top_groups=1),
+                                dict(num_groups=4, top_groups=5), dict(num_groups=4, top_groups=0),
+                                dict(num_groups=16, top_groups=1), dict(num_groups=4, top_groups=2, group_score_top=3)])
+def test_route_refuses_groups(cuda_pkg, kw):
+    with pytest.raises(cuda_pkg._lib.TJError, match="group"):
+        cuda_pkg.kernels.route_experts(torch.zeros(4, 64, device=DEV), 6, **kw)
+
+
+def test_gemm_refuses_widths(cuda_pkg):
+    k = cuda_pkg.kernels
+    r = k.route_experts(torch.zeros(4, 2, device=DEV), 1)
+    with pytest.raises(cuda_pkg._lib.TJError, match="multiples of 8"):
+        k.gemm_experts(torch.zeros(4, 12, dtype=torch.float16, device=DEV), torch.zeros(2, 8, 12, dtype=torch.float16, device=DEV),
+                       None, r, gather=True)
+    with pytest.raises(cuda_pkg._lib.TJError, match="multiples of 8"):
+        k.expert_ffn(torch.zeros(4, 16, dtype=torch.float16, device=DEV), torch.zeros(2, 12, 16, dtype=torch.float16, device=DEV),
+                     None, torch.zeros(2, 16, 12, dtype=torch.float16, device=DEV), None, r)
+    odd = torch.zeros(4 * 16 + 1, dtype=torch.float16, device=DEV)[1:].view(4, 16)
+    with pytest.raises(cuda_pkg._lib.TJError, match="aligned"):
+        k.gemm_experts(odd, torch.zeros(2, 8, 16, dtype=torch.float16, device=DEV), None, r, gather=True)
+
+
 def test_route_nan_rows(cuda_pkg):
     logits = _randn(_gen(2), 100, 40)
     clean = cuda_pkg.kernels.route_experts(logits, 3)
@@ -523,6 +563,49 @@ def test_sandwich_norm(cuda_pkg, rows, D, dtype, kind):
     _check_sandwich(cuda_pkg, x, b, pg, pb if beta else None, qg, qb if beta else None, kind)
     _check_sandwich(cuda_pkg, x, b, pg, None, None, None, kind, gate=_randn(g, D), scale=0.5)
     _check_sandwich(cuda_pkg, x, b, pg, pb, qg, None, kind, gate=_randn(g, rows, D, dtype=dtype), act="sigmoid", scale=-2.0)
+
+
+# Enough rows that they go through shared memory: every split of a row, whole
+# and partly filled, aligned and not; in place.
+@pytest.mark.parametrize("rows,D", [(700, 1), (700, 8), (1200, 31), (3000, 256), (700, 264), (700, 512), (701, 513),
+                                    (700, 1000), (700, 1032), (2000, 2048), (700, 2049), (350, 3000), (400, 4095), (900, 4096)])
+@pytest.mark.parametrize("dtype,kind", [(torch.float16, "layer"), (torch.bfloat16, "rms")])
+def test_sandwich_norm_many_rows(cuda_pkg, rows, D, dtype, kind):
+    g = _gen(rows + D)
+    x, b = _randn(g, rows, D, std=2.0), _randn(g, rows, D, dtype=dtype, std=1.5)
+    pg, pb = _affine(g, D)
+    qg, qb = _affine(g, D)
+    _check_sandwich(cuda_pkg, x, b, pg, pb, qg, qb, kind, gate=_randn(g, D), act="sigmoid", scale=0.5, live=rows - 3)
+    _check_sandwich(cuda_pkg, x, b, pg, None, None, None, kind, gate=_randn(g, rows, D, dtype=dtype), act="tanh")
+    _check_sandwich(cuda_pkg, x, b, pg, pb, qg, None, kind, gate=_randn(g, -(-rows // 64), D), per_gate=64)
+    s0, y0 = cuda_pkg.kernels.sandwich_norm(x, b, pg, pb, post_gamma=qg, kind=kind)
+    s, y = cuda_pkg.kernels.sandwich_norm(x, b, pg, pb, post_gamma=qg, kind=kind, sum_out=x, out=b)
+    assert s is x and y is b and torch.equal(s, s0) and torch.equal(y, y0)
+
+
+def test_sandwich_norm_of_more_experts_than_fit(cuda_pkg):
+    """16 and 32 experts' rows of 4096 columns: one row or none in shared memory."""
+    g = _gen(12)
+    for k, rows in ((6, 400), (16, 320), (32, 310)):
+        r = cuda_pkg.kernels.route_experts(_randn(g, rows, 40), k)
+        y = _randn(g, rows * k, 4096, dtype=torch.float16)
+        pg, pb = _affine(g, 4096)
+        _check_sandwich(cuda_pkg, _randn(g, rows, 4096), y, pg, pb, pg, pb, gate=_randn(g, 4096), routing=r)
+
+
+def test_sandwich_norm_past_32_bit_offsets(cuda_pkg):
+    """rows * D above 2^31 elements."""
+    g = _gen(13)
+    rows, D = 524_500, 4096
+    x = torch.empty(rows, D, device=DEV).normal_(generator=g)
+    b = torch.empty(rows, D, device=DEV, dtype=torch.float16).normal_(generator=g)
+    pg, pb = _affine(g, D)
+    s, y = cuda_pkg.kernels.sandwich_norm(x, b, pg, pb, post_gamma=pg)
+    assert s.numel() > 2**31
+    for lo in (0, 524_280, rows - 8):  # 2^31 / D = 524288
+        part = slice(lo, lo + 8)
+        s1, y1 = cuda_pkg.kernels.sandwich_norm(x[part].clone(), b[part].clone(), pg, pb, post_gamma=pg)
+        assert (s[part] - s1).abs().max() <= 1e-5 and torch.allclose(y[part].float(), y1.float(), rtol=2**-10, atol=1e-5)
 
 
 @pytest.mark.parametrize("D", [96, 1021, 2048])
