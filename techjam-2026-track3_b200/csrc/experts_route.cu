@@ -89,6 +89,7 @@ __device__ __forceinline__ double neg_inf<double>() { return __longlong_as_doubl
 // Reductions over the L lanes (a power of two) of a row.
 template <typename V>
 __device__ __forceinline__ V row_max(V v, int L) {
+#pragma unroll 1
   for (int o = L >> 1; o > 0; o >>= 1) {
     const V u = __shfl_xor_sync(0xffffffffu, v, o);
     v = u > v ? u : v;
@@ -97,12 +98,14 @@ __device__ __forceinline__ V row_max(V v, int L) {
 }
 template <typename V>
 __device__ __forceinline__ V row_sum(V v, int L) {
+#pragma unroll 1
   for (int o = L >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 // The greatest value and its expert, the lowest index among equals.
 template <typename V>
 __device__ __forceinline__ void row_best(V& v, int& e, int L) {
+#pragma unroll 1
   for (int o = L >> 1; o > 0; o >>= 1) {
     const V u = __shfl_xor_sync(0xffffffffu, v, o);
     const int f = __shfl_xor_sync(0xffffffffu, e, o);
@@ -123,6 +126,7 @@ __device__ __forceinline__ void push_top2(double& a, double& b, double x) {
 }
 template <typename V>
 __device__ __forceinline__ void row_top2(V& a, V& b, int L) {
+#pragma unroll 1
   for (int o = L >> 1; o > 0; o >>= 1) {
     const V c = __shfl_xor_sync(0xffffffffu, a, o), d = __shfl_xor_sync(0xffffffffu, b, o);
     push_top2(a, b, c);
@@ -415,8 +419,9 @@ __device__ void route_choose(const RouteParams& p, const float* bias, float bias
   __syncwarp();
 }
 
-// The weights of a tile's choices, L lanes to a row, lane j, j + L, ... of them.
-template <typename T>
+// The weights of a tile's choices, L lanes to a row, lane j, j + L, ... of them
+// (at most KL, all logits read at once).
+template <int KL, typename T>
 __device__ void route_weights(const RouteParams& p, const int* flags, const float* tops, const float* zs,
                               const uint16_t* chosen, int t0, int n, int live, int L) {
   const int row = (int)threadIdx.x / L, sub = (int)threadIdx.x & (L - 1);
@@ -425,42 +430,70 @@ __device__ void route_weights(const RouteParams& p, const int* flags, const floa
   const T* lg = static_cast<const T*>(p.logits) + grow * p.E;
   const uint16_t* mine = chosen + (on ? row : 0) * p.top_k;
   const bool here = on && grow < live;
-  const float top = on ? tops[row] : 0.f, z = on ? zs[row] : 1.f;
-  float cm = neg_inf<float>(), sum = 0.f, near = 0.f;
-  if (p.renorm) {
-    if (here)
-#pragma unroll 4
-      for (int j = sub; j < p.top_k; j += L)
-        if (mine[j] != kNoChoice) cm = fmaxf(cm, route_load(lg + mine[j]));
-    cm = row_max(cm, L);
-    if (!(cm > neg_inf<float>())) cm = 0.f;
-    if (here)
-#pragma unroll 4
-      for (int j = sub; j < p.top_k; j += L)
-        if (mine[j] != kNoChoice) {
-          const float c = route_load(lg + mine[j]);
-          near += expf(c - cm);  // softmax: its denominator cancels
-          if (p.sigmoid) sum += 1.f / (1.f + expf(-c));
-        }
-    near = row_sum(near, L);
-    sum = row_sum(sum, L);
+  int e[KL];
+  float c[KL];
+#pragma unroll
+  for (int i = 0; i < KL; ++i) {
+    const int j = sub + i * L;
+    e[i] = here && j < p.top_k && mine[j] != kNoChoice ? mine[j] : -1;
+    c[i] = e[i] >= 0 ? route_load(lg + e[i]) : neg_inf<float>();
   }
-  // Far below zero the sigmoids underflow, their ratios (those of exp) do not.
-  const bool ratio = p.renorm && (!p.sigmoid || sum < 1e-30f);
-  const float scale = !p.renorm ? p.weight_scale : (ratio ? (near > 0.f ? p.weight_scale / near : 0.f) : p.weight_scale / sum);
-  const bool bad = here && flags[row] != 0;
-  if (on)
-#pragma unroll 4
-    for (int j = sub; j < p.top_k; j += L) {
-      const int e = here && mine[j] != kNoChoice ? mine[j] : -1;
-      float w = 0.f;
-      if (e >= 0) {
-        const float c = route_load(lg + e);
-        w = ratio ? expf(c - cm) : (p.sigmoid ? 1.f / (1.f + expf(-c)) : expf(c - top) / z);
-      }
-      p.experts[grow * p.top_k + j] = e;
-      p.weights[grow * p.top_k + j] = bad ? __int_as_float(0x7fc00000) : w * scale;
+  float scale = p.weight_scale;
+  if (p.sigmoid) {
+    float sum = 0.f, cm = neg_inf<float>();
+#pragma unroll
+    for (int i = 0; i < KL; ++i) {
+      cm = fmaxf(cm, c[i]);
+      c[i] = e[i] >= 0 ? __fdividef(1.f, 1.f + expf(-c[i])) : 0.f;
+      sum += c[i];
     }
+    if (p.renorm) {
+      sum = row_sum(sum, L);
+      // Far below zero the sigmoids underflow, their ratios (those of exp) do not.
+      if (__any_sync(0xffffffffu, sum < 1e-30f)) {
+        cm = row_max(cm, L);
+        float far[KL], total = 0.f;
+#pragma unroll
+        for (int i = 0; i < KL; ++i) {
+          far[i] = e[i] >= 0 ? expf(route_load(lg + e[i]) - cm) : 0.f;
+          total += far[i];
+        }
+        total = row_sum(total, L);
+        if (sum < 1e-30f) {
+          sum = total;
+#pragma unroll
+          for (int i = 0; i < KL; ++i) c[i] = far[i];
+        }
+      }
+      scale = sum > 0.f ? scale / sum : 0.f;
+    }
+  } else {
+    float top = on ? tops[row] : 0.f, z = on ? zs[row] : 1.f;
+    if (p.renorm) {  // the denominator of the softmax cancels
+      top = neg_inf<float>();
+#pragma unroll
+      for (int i = 0; i < KL; ++i) top = fmaxf(top, c[i]);
+      top = row_max(top, L);
+      z = 0.f;
+    }
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < KL; ++i) {
+      c[i] = e[i] >= 0 ? expf(c[i] - top) : 0.f;
+      sum += c[i];
+    }
+    if (p.renorm) z = row_sum(sum, L);
+    scale = z > 0.f ? scale / z : 0.f;
+  }
+  if (here && flags[row] != 0) scale = __int_as_float(0x7fc00000);
+#pragma unroll
+  for (int i = 0; i < KL; ++i) {
+    const int j = sub + i * L;
+    if (on && j < p.top_k) {
+      p.experts[grow * p.top_k + j] = e[i];
+      p.weights[grow * p.top_k + j] = c[i] * scale;
+    }
+  }
 }
 
 // ---- plan ---------------------------------------------------------------------
@@ -597,7 +630,7 @@ __global__ void __launch_bounds__(KL > 16 ? 512 : kRouteThreads) route_kernel(co
         const int units = p.E / W;  // of a row
         int row = (int)threadIdx.x / units, u = (int)threadIdx.x % units;
         const int row_step = (int)blockDim.x / units, u_step = (int)blockDim.x % units;
-#pragma unroll 4
+#pragma unroll 8
         for (int i = (int)threadIdx.x * W; i < items; i += (int)blockDim.x * W) {
           float x[W];
           if (i < read) {
@@ -639,7 +672,7 @@ __global__ void __launch_bounds__(KL > 16 ? 512 : kRouteThreads) route_kernel(co
         stage(std::integral_constant<int, 1>());
       __syncthreads();
       route_choose<KL, T>(p, bias, bias_max, xs, p.pitch, flags, strengths, tops, zs, maybe, chosen, t0, n, p.lanes);
-      route_weights<T>(p, flags, tops, zs, chosen, t0, n, live, p.lanes);
+      route_weights<KL, T>(p, flags, tops, zs, chosen, t0, n, live, p.lanes);
       __syncthreads();
       for (int i = threadIdx.x; i < n * p.top_k; i += (int)blockDim.x)
         if (chosen[i] != kNoChoice) atomicAdd(hist + chosen[i], 1);
