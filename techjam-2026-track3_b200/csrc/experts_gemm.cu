@@ -68,9 +68,10 @@ struct XpParams {
   void* out;                // [slots][N]
   int slots, rows, E, N, K;
   // 1: the plan and the weights were there before the preceding kernel of the
-  // stream started (tj_expert_ffn's FFN-out: FFN-in has waited for the router),
-  // so only what reads or writes activations waits for that kernel, and an SM
-  // that is done with it loads weights while the others finish.
+  // stream let this one start (FFN-out after FFN-in, FFN-in after the permuted
+  // copy: those have waited for the router), so only what reads or writes
+  // activations waits for that kernel, and an SM that is done with it loads
+  // weights while the others finish.
   int plan_ready;
   int splits;               // parts of K; part i writes plane i of out [splits][slots][N]
 };
@@ -246,6 +247,7 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
     }
   }
   if (!p.plan_ready) pdl_wait();
+  pdl_trigger();  // the next kernel's CTAs take the SMs as this one's leave them
   const int m_tiles = (p.N + Cfg::kFeatures - 1) / Cfg::kFeatures;
   // Offsets, held inside [0, slots] whatever the plan says.
   for (int e = threadIdx.x; e <= p.E; e += kXpThreads) {
@@ -530,7 +532,6 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
   }
 
   __syncwarp();
-  pdl_trigger();
   tc_fence_before();
   if constexpr (kPair)
     cluster_sync();  // the peer no longer reads this CTA's shared memory or barriers
@@ -761,6 +762,7 @@ int launch_experts_gemm(const ExpertGemmArgs& a, cudaStream_t stream) {
       int rc = launch_expert_gather(a, a.workspace, stream);
       if (rc) return rc;
       g.a = a.workspace;
+      kp.plan_ready = 1;
       g.a_rows = a.slots;
     }
     return launch_experts_gemm_bn<true, 256, false>(g, kp, stream);
