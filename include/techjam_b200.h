@@ -348,7 +348,7 @@ TJ_API int tj_expert_ffn(const void* a, int dtype, const void* w_in, const float
  * is (gate_map ? gate_map[r] : r) / rows_per_gate: gate [1, D] with
  * rows_per_gate >= rows for a gate per channel, rows_per_gate = seq_len for
  * one per sample, 1 for one per row.  d_model up to 32768 (8192 when it is not
- * a multiple of 4, an fp32 pointer not 16-byte or a 16-bit one not 8-byte aligned).  sum_out may be x
+ * a multiple of 8 or a pointer is not 16-byte aligned).  sum_out may be x
  * itself when row_map is NULL.  A row map entry or gate row outside its buffer
  * is recorded as a device error and the row is left out. */
 typedef struct tj_sandwich_desc {

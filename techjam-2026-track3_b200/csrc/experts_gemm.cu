@@ -22,10 +22,15 @@
 // features x up to 256 tokens, each CTA loading half of either operand, 32 KB
 // per K step of 64 instead of 48 KB; both CTAs' loads arrive on the leader's
 // barrier, as in the dense GEMM.  Pairs read consecutive slots only: a row
-// gather takes 73 cycles of the TMA unit, and cp.async gathers wait for a
-// proxy fence (about 1800 cycles with copies in flight) per stage.  48002
-// slots, D 1024, F 4096: 1590 us by TMA gathers, 620 us by cp.async, 310 us
-// from a permuted copy, which expert_gather_kernel writes in about 30 us.
+// gather takes 73 cycles of the TMA unit, and gathers by cp.async or through
+// registers wait for a proxy fence per stage, which waits for what is in flight
+// (about 1800 cycles).  48002 slots, D 1024, F 4096, FFN-in without GELU: 1590 us
+// by TMA gathers, 620 by cp.async, 830 through registers, 320 from a permuted
+// copy, which expert_gather_kernel writes in 25 us.
+// What bounds it: many rows per expert, the tensor cores under the power cap
+// (48000 x 1024 x 4096: 311 us, 1.29 PFLOP/s, where cuBLAS takes 291 us for the
+// product with one weight; GELU adds 36 us to FFN-in); few rows, the weights'
+// bytes (33 tokens x 4 of 64 experts: 223 MB in 41 us, 5.5 TB/s).
 // The FFN-out of tj_expert_ffn leaves fp32 (expert_combine sums it).  With few
 // tiles its K is cut into `splits` parts, each its own tile with its own plane
 // of the output, which the combine adds up: no CTA waits for another, and one
