@@ -54,7 +54,7 @@ template <bool kPair, int BN>
 struct XpCfg {
   static constexpr int kXRows = kPair ? BN / 2 : BN;         // token rows of this CTA
   static constexpr int kFeatures = kPair ? 2 * kBM : kBM;    // of a tile
-  static constexpr int kStages = kPair ? 6 : (BN >= 64 ? 7 : 9);
+  static constexpr int kStages = kPair ? 6 : 9;
   static constexpr uint32_t kWBytes = kBM * kBK * 2;
   static constexpr uint32_t kXBytes = kXRows * kBK * 2;
   static constexpr uint32_t kStageBytes = kWBytes + kXBytes;
