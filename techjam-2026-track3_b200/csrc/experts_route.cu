@@ -122,10 +122,6 @@ __device__ __forceinline__ void push_top2(float& a, float& b, float x) {
   b = fmaxf(b, fminf(a, x));
   a = fmaxf(a, x);
 }
-__device__ __forceinline__ void push_top2(double& a, double& b, double x) {
-  b = fmax(b, fmin(a, x));
-  a = fmax(a, x);
-}
 template <typename V>
 __device__ __forceinline__ void row_top2(V& a, V& b, int L) {
 #pragma unroll 1
@@ -146,61 +142,98 @@ __device__ __forceinline__ float route_load(const T* p) {
   return (float)__ldg(p);
 }
 
-// A row's choices in fp64, a warp to the row: lane j writes choice j.  m: the
-// row's greatest logit or 0.
+// Unsigned keys ordered like the doubles they come from (no NaN; -0 joined to
+// +0); 0 for a closed expert.
+__device__ __forceinline__ unsigned long long double_order(double x) {
+  const long long b = __double_as_longlong(x + 0.0);
+  return (unsigned long long)(b ^ ((b >> 63) | (long long)0x8000000000000000ull));
+}
+__device__ __forceinline__ double order_double(unsigned long long k) {
+  return __longlong_as_double((long long)((k >> 63) ? k ^ 0x8000000000000000ull : ~k));
+}
+// The warp's greatest key and the lowest index that has it (kNoIndex if all are closed).
+constexpr unsigned kNoIndex = 0xffffffffu;
+__device__ __forceinline__ unsigned warp_best(unsigned long long& key, unsigned index) {
+  const unsigned hi = __reduce_max_sync(0xffffffffu, (unsigned)(key >> 32));
+  const unsigned lo = __reduce_max_sync(0xffffffffu, (unsigned)(key >> 32) == hi ? (unsigned)key : 0u);
+  const unsigned long long best = (unsigned long long)hi << 32 | lo;
+  const unsigned at = __reduce_min_sync(0xffffffffu, key == best && best != 0 ? index : kNoIndex);
+  key = best;
+  return at;
+}
+
+// A row's choices in fp64, a warp to the row.  m: the row's greatest logit or 0.
 template <typename T>
 __device__ __noinline__ void route_row_exact(const RouteParams& p, const float* bias, const T* lg, float m, int lane,
                                              uint16_t* chosen) {
   constexpr int V = kRouteMaxExperts / 32;
   const int n = (p.E + 31) / 32;  // of the V places used
-  double v[V];                    // of experts i * 32 + lane
-  double z = 0.0;
+  unsigned long long v[V];        // of experts i * 32 + lane
+  double z = 1.0;
+  if (!p.sigmoid) {
+    z = 0.0;
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      const int e = i * 32 + lane;
+      if (e < p.E) z += exp((double)route_load(lg + e) - (double)m);  // 0 for a closed expert
+    }
+    z = row_sum(z, 32);
+  }
+#pragma unroll 1
   for (int i = 0; i < n; ++i) {
     const int e = i * 32 + lane;
     const double x = e < p.E ? (double)route_load(lg + e) : neg_inf<double>();
-    v[i] = exp(p.sigmoid ? -x : x - (double)m);
-    z += v[i];
-    if (!(x > neg_inf<double>())) v[i] = neg_inf<double>();
-  }
-  if (!p.sigmoid) z = row_sum(z, 32);
-  for (int i = 0; i < n; ++i) {
-    const int e = i * 32 + lane;
-    if (v[i] > neg_inf<double>())
-      v[i] = (p.sigmoid ? 1.0 / (1.0 + v[i]) : v[i] / z) + (double)(p.bias ? bias[e] : 0.f);
+    const double a = exp(p.sigmoid ? -x : x - (double)m);
+    const double w = (p.sigmoid ? 1.0 / (1.0 + a) : a / z) + (double)(p.bias && e < p.E ? bias[e] : 0.f);
+    v[i] = x > neg_inf<double>() && w > neg_inf<double>() ? double_order(w) : 0ull;
   }
   if (p.groups > 1) {
     const int per = p.E / p.groups;
     double strength = neg_inf<double>();  // of group `lane`
+#pragma unroll 1
     for (int g = 0; g < p.groups; ++g) {
-      double a = neg_inf<double>(), b = neg_inf<double>();
+      unsigned long long a = 0, b = 0;  // the lane's greatest two of the group
+#pragma unroll 1
       for (int i = 0; i < n; ++i) {
         const int e = i * 32 + lane;
-        push_top2(a, b, e >= g * per && e < (g + 1) * per ? v[i] : neg_inf<double>());
+        const unsigned long long k = e >= g * per && e < (g + 1) * per ? v[i] : 0ull;
+        b = k > a ? a : (k > b ? k : b);
+        a = k > a ? k : a;
       }
-      row_top2(a, b, 32);
-      if (lane == g) strength = group_strength(a, b, p.group_top);
+      unsigned long long first = a;
+      const unsigned owner = warp_best(first, lane);
+      double s = first != 0 ? order_double(first) : neg_inf<double>();
+      if (p.group_top == 2) {
+        unsigned long long second = lane == owner ? b : a;
+        warp_best(second, lane);
+        if (second != 0) s += order_double(second);
+      }
+      if (lane == g) strength = s;
     }
     int above = 0;
+#pragma unroll 1
     for (int g = 0; g < p.groups; ++g) {
       const double o = __shfl_sync(0xffffffffu, strength, g);
       above += o > strength || (o == strength && g < lane);
     }
     const unsigned kept = __ballot_sync(0xffffffffu, lane < p.groups && above < p.top_groups);
+#pragma unroll 1
     for (int i = 0; i < n; ++i)
-      if (!((kept >> (((i * 32 + lane) / per) & 31)) & 1u)) v[i] = neg_inf<double>();
+      if (!((kept >> (((i * 32 + lane) / per) & 31)) & 1u)) v[i] = 0ull;
   }
+#pragma unroll 1
   for (int j = 0; j < p.top_k; ++j) {
-    double best = neg_inf<double>();
-    int e = lane;
+    unsigned long long best = 0;
+    unsigned e = lane;
+#pragma unroll 1
     for (int i = 0; i < n; ++i)
       if (v[i] > best) {
         best = v[i];
-        e = i * 32 + lane;
+        e = (unsigned)(i * 32 + lane);
       }
-    row_best(best, e, 32);
-    for (int i = 0; i < n; ++i)
-      if (e == i * 32 + lane) v[i] = neg_inf<double>();
-    if (lane == 0) chosen[j] = best > neg_inf<double>() ? (uint16_t)e : kNoChoice;
+    const unsigned at = warp_best(best, e);
+    if (at != kNoIndex && (at & 31u) == (unsigned)lane) v[at >> 5] = 0ull;
+    if (lane == 0) chosen[j] = at != kNoIndex ? (uint16_t)at : kNoChoice;
   }
 }
 
@@ -422,10 +455,10 @@ __device__ void route_choose(const RouteParams& p, const float* bias, float bias
 }
 
 // The weights of a tile's choices, L lanes to a row, lane j, j + L, ... of them
-// (at most KL, all logits read at once).
+// (at most KL, all logits read at once), to out[row * top_k + j].
 template <int KL, typename T>
 __device__ void route_weights(const RouteParams& p, const int* flags, const float* tops, const float* zs,
-                              const uint16_t* chosen, int t0, int n, int live, int L) {
+                              const uint16_t* chosen, float* out, int t0, int n, int live, int L) {
   const int row = (int)threadIdx.x / L, sub = (int)threadIdx.x & (L - 1);
   const bool on = row < n;
   const int64_t grow = t0 + (on ? row : 0);
@@ -491,10 +524,7 @@ __device__ void route_weights(const RouteParams& p, const int* flags, const floa
 #pragma unroll
   for (int i = 0; i < KL; ++i) {
     const int j = sub + i * L;
-    if (on && j < p.top_k) {
-      p.experts[grow * p.top_k + j] = e[i];
-      p.weights[grow * p.top_k + j] = c[i] * scale;
-    }
+    if (on && j < p.top_k) out[row * p.top_k + j] = c[i] * scale;
   }
 }
 
@@ -674,10 +704,17 @@ __global__ void __launch_bounds__(KL > 16 ? 512 : kRouteThreads) route_kernel(co
         stage(std::integral_constant<int, 1>());
       __syncthreads();
       route_choose<KL, T>(p, bias, bias_max, xs, p.pitch, flags, strengths, tops, zs, maybe, chosen, t0, n, p.lanes);
-      route_weights<KL, T>(p, flags, tops, zs, chosen, t0, n, live, p.lanes);
       __syncthreads();
-      for (int i = threadIdx.x; i < n * p.top_k; i += (int)blockDim.x)
-        if (chosen[i] != kNoChoice) atomicAdd(hist + chosen[i], 1);
+      // the values are done with: the weights take their place on the way out
+      route_weights<KL, T>(p, flags, tops, zs, chosen, xs, t0, n, live, p.lanes);
+      __syncthreads();
+      const int64_t at = (int64_t)t0 * p.top_k;
+      for (int i = threadIdx.x; i < n * p.top_k; i += (int)blockDim.x) {
+        const uint16_t e = chosen[i];
+        if (e != kNoChoice) atomicAdd(hist + e, 1);
+        p.experts[at + i] = e != kNoChoice ? e : -1;
+        p.weights[at + i] = xs[i];
+      }
       __syncthreads();
     }
   } else {
