@@ -25,7 +25,7 @@
 // gives each row L lanes, as many as it has threads for: one when the rows are
 // many, so that no instruction is spent on lanes agreeing, 32 for a few. Each
 // lane keeps the sorted best of its experts (i L + its number), then the lanes'
-// lists are merged.  90077 rows of 64 experts in groups, router and plan: 48 us;
+// lists are merged.  90077 rows of 64 experts in groups, router and plan: 47 us;
 // a warp per row took 243 us, 8 lanes a row with eight experts each in registers
 // 80 us.  Bound by instructions and their latency (16.3 M for 60000 rows), not by
 // the 33 MB it moves (5 us).
