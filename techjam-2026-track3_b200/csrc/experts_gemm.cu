@@ -41,6 +41,8 @@
 #include "common.cuh"
 #include "internal.h"
 
+#include <cstddef>
+
 namespace tj {
 
 constexpr int kXpThreads = 384;
@@ -122,6 +124,20 @@ __device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uin
                : "memory");
 }
 
+// Counts `bytes` as arrived on a barrier, without a copy.
+__device__ __forceinline__ void mbar_complete_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ int ld_shared_cluster(uint32_t cluster_addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_shared_cluster(uint32_t cluster_addr, int v) {
+  asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+}
+
 // Operand formats of the instruction descriptor (bits 7-9 and 10-12).
 template <typename T>
 struct XpType;
@@ -196,6 +212,43 @@ struct XpWalk {
   }
 };
 
+// K steps whose loads this CTA's producers have sent, and the bytes of the token
+// loads of the last step in each stage.
+struct XpSent {
+  int weights, tokens;
+  int token_bytes[9];
+};
+
+// After a wait has run out (or an earlier kernel's error has kept a producer
+// from starting) the producers, in a pair those of both CTAs, may have stopped
+// at different K steps.  Waits until all loads sent have landed: the steps that
+// not every producer reached get the arrivals and bytes that will not come,
+// then each completes when its copies have.  A producer is at most S steps
+// ahead of the products, which need every producer's loads, so only the last S
+// steps can be open.  One thread of the leader, when all producers have left.
+template <bool kPair, int S, uint32_t kWBytes>
+__device__ void experts_gemm_drain(uint64_t* full, XpSent* sent) {
+  const uint32_t peer = kPair ? mapa_shared(smem_u32(sent), 1) : 0;
+  const int w0 = sent->weights, x0 = sent->tokens;
+  const int w1 = kPair ? ld_shared_cluster(peer + offsetof(XpSent, weights)) : w0;
+  const int x1 = kPair ? ld_shared_cluster(peer + offsetof(XpSent, tokens)) : x0;
+  const int last = max(max(w0, x0), max(w1, x1));
+  for (int i = max(0, last - S); i < last; ++i) {
+    const int s = i % S;
+    const uint32_t bar = smem_u32(full + s);
+    if (i >= w0)
+      mbar_arrive_expect_tx(bar, kPair && i < w1 ? kWBytes : 0u);
+    else if (kPair && i >= w1)
+      mbar_complete_tx(bar, kWBytes);
+    if (i >= x0)
+      mbar_arrive_expect_tx(
+          bar, kPair && i < x1 ? ld_shared_cluster(peer + offsetof(XpSent, token_bytes) + 4 * s) : 0);
+    else if (kPair && i >= x1)
+      mbar_complete_tx(bar, sent->token_bytes[s]);
+    drain_wait(bar, (uint32_t)(i / S) & 1u);
+  }
+}
+
 // Out: T, or float for the fp32 planes.
 template <bool kPair, int BN, bool kGelu, bool kGather, typename T, typename Out>
 __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const CUtensorMap& tmX,
@@ -213,6 +266,8 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
   // bars: full[S] (leader's used), empty[S], tfull[2], tempty[2] (leader's used), final
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 5);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  XpSent* sent = reinterpret_cast<XpSent*>(tmem_slot + 2);
+  static_assert((2 * S + 5) * 8 + 8 + sizeof(XpSent) <= 512 && S <= 9, "the barriers' 512 bytes");
   int* first = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(bars) + 512);  // [E+1]
   int* tiles = first + p.E + 1;                                                // [E+1]
 
@@ -237,6 +292,7 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
     }
     mbar_init(final_bar, 1);
     *abort_flag = device_failed() ? 1 : 0;
+    sent->weights = sent->tokens = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tmW);
     tma_prefetch_desc(&tmX);
@@ -286,8 +342,7 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
       Walk walk(first, tiles, p.E, m_tiles, p.splits, tile_step);
       int stage = 0;
       uint32_t phase = 0;
-      int last_parity[S];
-      for (int s = 0; s < S; ++s) last_parity[s] = -1;
+      int steps = 0;
       for (int t = tile0; t < walk.total && !*abort_flag; t += tile_step) {
         const XpTile tile = walk.at(t);
         if (tile.n <= 0) continue;
@@ -299,25 +354,22 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
             tma_load_3d_pair(dst, &tmW, mapa_shared(full_bar(stage), 0), kb * kBK, tile.m0 + rank * kBM, tile.e);
           else
             tma_load_3d(dst, &tmW, full_bar(stage), kb * kBK, tile.m0, tile.e);
-          last_parity[stage] = (int)phase;
+          ++steps;
           if (++stage == S) {
             stage = 0;
             phase ^= 1;
           }
         }
       }
-      // Every load of both producers (and of the peer) has landed once the
-      // leader's barriers complete.
-      if (leader)
-        for (int s = 0; s < S; ++s)
-          if (last_parity[s] >= 0) drain_wait(full_bar(s), (uint32_t)last_parity[s]);
+      sent->weights = steps;
     }
   } else if (warp == 1) {
     if (p.plan_ready) pdl_wait();
     Walk walk(first, tiles, p.E, m_tiles, p.splits, tile_step);
     int stage = 0;
     uint32_t phase = 0;
-    bool ok = true;
+    int steps = 0;
+    bool ok = !__any_sync(0xffffffffu, *abort_flag);  // the first waits do not look at it
     for (int t = tile0; t < walk.total && ok; t += tile_step) {
       const XpTile tile = walk.at(t);
       if (tile.n <= 0) continue;
@@ -339,6 +391,7 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const uint32_t dst = smem_u32(sX + stage * Cfg::kXBytes) + lane * (kRows * 128);
+        if (lane == 0) sent->token_bytes[stage] = loads * kRows * 128;
         if (leader && lane == 0) mbar_arrive_expect_tx(full_bar(stage), (uint32_t)(kCtas * loads * kRows * 128));
         __syncwarp();
         if (lane < loads) {
@@ -349,12 +402,14 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
           else
             tma_load_2d(dst, &tmX, full_bar(stage), kb * kBK, row[0]);
         }
+        ++steps;
         if (++stage == S) {
           stage = 0;
           phase ^= 1;
         }
       }
     }
+    if (lane == 0) sent->tokens = steps;
   } else if (warp == 2) {
     if (leader && lane == 0) {
       Walk walk(first, tiles, p.E, m_tiles, p.splits, tile_step);
@@ -432,7 +487,7 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
       const XpTile tile = walk.at(t);
       if (tile.n <= 0) continue;
       const int f0 = tile.m0 + rank * kBM + quarter * 32;  // this warp's 32 features
-      if (!mbar_wait(tfull_bar(acc), acc_phase, abort_flag, 254)) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(tfull_bar(acc), acc_phase, abort_flag, 254))) break;
       tc_fence_after();
       const uint32_t t_row = tmem_base + (uint32_t)(acc * BN) + ((uint32_t)(quarter * 32) << 16);
       const float* bias = (p.bias && tile.split == 0) ? p.bias + (int64_t)tile.e * p.N : nullptr;
@@ -537,11 +592,22 @@ __device__ __forceinline__ void experts_gemm_body(const CUtensorMap& tmW, const 
   }
 
   __syncwarp();
+  if (kPair && *abort_flag) st_shared_cluster(mapa_shared(smem_u32((const int*)abort_flag), rank ^ 1), 1);
   tc_fence_before();
-  if constexpr (kPair)
-    cluster_sync();  // the peer no longer reads this CTA's shared memory or barriers
-  else
-    __syncthreads();
+  auto meet = [&]() {
+    if constexpr (kPair)
+      cluster_sync();  // the peer no longer reads this CTA's shared memory or barriers
+    else
+      __syncthreads();
+  };
+  meet();
+  // The products have waited for every load, unless something gave up.  The flag
+  // is the same in both CTAs of a pair now.
+  if (*abort_flag) {
+    if (leader && threadIdx.x == 0) experts_gemm_drain<kPair, S, Cfg::kWBytes>(bars, sent);
+    __syncwarp();
+    meet();
+  }
   if (warp == 2) {
     tc_fence_after();
     if constexpr (kPair)

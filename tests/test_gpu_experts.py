@@ -799,3 +799,64 @@ def test_block_captured_and_on_two_streams(cuda_pkg):
         for a, b in zip(outputs(got), want[i]):
             assert torch.equal(a, b)
     assert cuda_pkg._lib.device_status(torch.cuda.current_stream().cuda_stream) == [0, 0, 0, 0]
+
+
+# ---- given up on -------------------------------------------------------------------
+# Products of few rows (TMA row gathers) and of many (CTA pairs after the permuted
+# copy), with more K steps than stages.
+def _products(k, g, rows, E=4, D=1024, F=768):
+    r = k.route_experts(_randn(g, rows, E), 2)
+    a = _randn(g, rows, D, dtype=torch.float16)
+    w_in, w_out = _weights(g, E, F, D, torch.float16), _weights(g, E, D, F, torch.float16)
+    h = torch.empty(rows * 2, F, dtype=torch.float16, device=DEV)
+
+    def run(fill=None):
+        if fill is not None:
+            h.fill_(fill)
+        k.gemm_experts(a, w_in, None, r, gather=True, gelu=True, out=h)
+        y = k.gemm_experts(h, w_out, None, r, gather=False)
+        return h, y, k.expert_ffn(a, w_in, None, w_out, None, r)
+
+    return run
+
+
+@pytest.mark.parametrize("rows", [20, 1500])
+def test_products_after_a_recorded_error(cuda_pkg, rows):
+    """Until the status is read the products load and write nothing; then they are as before."""
+    L, k = cuda_pkg._lib, cuda_pkg.kernels
+    run = _products(k, _gen(rows), rows)
+    want = [t.clone() for t in run()]
+    L.set_sync_check(False)
+    stream = torch.cuda.current_stream().cuda_stream
+    for _ in range(5):
+        k.expert_plan(torch.full((rows, 2), 9, dtype=torch.int32, device=DEV), torch.ones(rows, 2, device=DEV), 8)
+        h, _, _ = run(fill=7.0)
+        with pytest.raises(L.TJError, match="outside"):
+            L.device_status(stream)
+        assert (h == 7).all()
+        for got, ref in zip(run(), want):
+            assert torch.equal(got, ref)
+        assert L.device_status(stream) == [0, 0, 0, 0]
+
+
+@pytest.mark.parametrize("rows", [20, 1500])
+def test_products_whose_waits_run_out(cuda_pkg, rows):
+    """A wait limit of 1 ns: producers stop at different steps, everything sent
+    lands, and the next products are as before."""
+    L, k = cuda_pkg._lib, cuda_pkg.kernels
+    lib = L.load()
+    run = _products(k, _gen(rows), rows)
+    want = [t.clone() for t in run()]
+    L.set_sync_check(False)
+    stream = torch.cuda.current_stream().cuda_stream
+    for _ in range(20):
+        L.check(lib.tj_debug_set_wait_limit_ns(1), "debug_set_wait_limit_ns")
+        try:
+            run()
+            with pytest.raises(L.TJError, match="time limit"):
+                L.device_status(stream)
+        finally:
+            L.check(lib.tj_debug_set_wait_limit_ns(0), "debug_set_wait_limit_ns")
+        for got, ref in zip(run(), want):
+            assert torch.equal(got, ref)
+        assert L.device_status(stream) == [0, 0, 0, 0]
