@@ -300,9 +300,18 @@ __device__ void route_choose(const RouteParams& p, const float* bias, float bias
     for (int e = sub; e < E; e += L) m = fmaxf(m, x[e * pitch]);
     m = row_max(m, L);
     top = m > neg_inf<float>() ? m : 0.f;  // a closed row's exponentials are 0, not NaN
+    // Blocks of 16 in four parts: one after the other a lane's up to 193 terms
+    // could all round the same way, 1.1e-5 of the sum.
     z = 0.f;
-#pragma unroll 4
-    for (int e = sub; e < E; e += L) z += expf(x[e * pitch] - top);
+    for (int e0 = sub; e0 < E; e0 += 16 * L) {
+      float part[4] = {};
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int e = e0 + i * L;
+        if (e < E) part[i & 3] += expf(x[e * pitch] - top);
+      }
+      z += (part[0] + part[1]) + (part[2] + part[3]);
+    }
     z = row_sum(z, L);
   }
   const float zi = 1.f / z;
@@ -311,11 +320,13 @@ __device__ void route_choose(const RouteParams& p, const float* bias, float bias
     // |error of v| <= |error of s| + 2^-24 |v|.  Sigmoid: e = 2^(-x log2 e) with
     // the product rounded (|x| 2^-23 relative) and ex2 within 2 ulp, 1 + e rounded,
     // the quotient within 2 ulp: s (1 - s) (2^-22 + |x| 2^-23) + s (2^-24 + 2^-22),
-    // at most 4.2e-7.  Softmax: the sum of up to 512 terms (at most 64 in order,
-    // then the lanes) is within 69 ulp (2^-24 each), expf within 2 ulp, two more
-    // roundings: 5e-6 of the greatest score, 1 / z.
+    // at most 4.2e-7.  Softmax, in 2^-24 of the greatest score, 1 / z: the sum of
+    // n = E / L terms to a lane 5 (a block of 16) + n / 16 + 1 (blocks) + 5 (lanes);
+    // expf within 2 ulp 4, in the sum and in the score; x - top rounded, d 2^-24
+    // of exp(-d): log E <= 6.3 in the sum, 0.4 in the score; 1 / z and the product 2.
     const float smax = p.sigmoid ? 1.f : zi;
-    err = (p.sigmoid ? 4.2e-7f : 5e-6f * smax) + 6e-8f * (smax + bias_max);
+    const float terms = 28.f + 0.0625f * (float)(E / L + 1);
+    err = (p.sigmoid ? 4.2e-7f : 6e-8f * terms * smax) + 6e-8f * (smax + bias_max);
   }
   // Value of expert e, in place of its logit.
   const bool set = by_value && on && !bad;
@@ -511,13 +522,13 @@ __device__ void route_weights(const RouteParams& p, const int* flags, const floa
       top = row_max(top, L);
       z = 0.f;
     }
-    float sum = 0.f;
+    float sum[2] = {};  // of few terms each, like the denominator
 #pragma unroll
     for (int i = 0; i < KL; ++i) {
       c[i] = e[i] >= 0 ? expf(c[i] - top) : 0.f;
-      sum += c[i];
+      sum[i & 1] += c[i];
     }
-    if (p.renorm) z = row_sum(sum, L);
+    if (p.renorm) z = row_sum(sum[0] + sum[1], L);
     scale = z > 0.f ? scale / z : 0.f;
   }
   if (here && flags[row] != 0) scale = __int_as_float(0x7fc00000);

@@ -860,3 +860,50 @@ def test_products_whose_waits_run_out(cuda_pkg, rows):
         for got, ref in zip(run(), want):
             assert torch.equal(got, ref)
         assert L.device_status(stream) == [0, 0, 0, 0]
+
+
+# ---- routing: rows of many terms, biases far apart, scores that saturate ---------------
+def _peaked(rows, E):
+    """Softmax rows whose denominator, summed one after the other in fp32, rounds up at every term."""
+    logits = torch.full((rows, E), math.log(1.01 * 2.0**-24), device=DEV)
+    logits[:, 0] = 0.0
+    return logits
+
+
+# As many terms to a lane as there are (rows many, so few lanes to each): top_k up to
+# 16 and above (half the threads), one chunk of rows and many.
+@pytest.mark.parametrize("rows,E,k", [(19092, 384, 17), (15000, 512, 24), (30000, 88, 17), (14000, 512, 8), (60, 512, 32)])
+def test_route_biased_softmax_of_many_terms(cuda_pkg, rows, E, k):
+    logits = _peaked(rows, E)
+    p = torch.softmax(logits[0].double(), 0)
+    bias = -1.0 - 0.01 * torch.arange(E, device=DEV)
+    bias[0] = 0.0
+    for below in (3e-7, -3e-7):  # how far expert 1 lies below expert 0
+        bias[1] = float(p[0] - p[1] - below)
+        r = _check_route(cuda_pkg, logits, k, bias=bias)
+        assert int(r.experts[0, 0]) == (0 if below > 0 else 1)
+
+
+# Tolerance of _check_route: 32 * 2^-24.  The denominator is summed in blocks of 16
+# in four parts (5 roundings), at most 13 blocks, and over the lanes (5); expf within
+# 2 ulp (4 * 2^-24), the exponents' differences are exact here, two more roundings.
+@pytest.mark.parametrize("rows,E,k", [(19092, 384, 17), (15000, 512, 32), (14000, 512, 8), (30000, 88, 20), (60, 512, 32)])
+@pytest.mark.parametrize("renorm", [False, True])
+def test_route_weights_of_many_terms(cuda_pkg, rows, E, k, renorm):
+    _check_route(cuda_pkg, _peaked(rows, E), k, renorm=renorm)
+    flat = torch.zeros(rows, E, device=DEV)
+    flat[:, 1] = 1.0
+    _check_route(cuda_pkg, flat, k, renorm=renorm)
+    _check_route(cuda_pkg, _peaked(rows, E), k, "sigmoid", renorm=renorm)
+
+
+@pytest.mark.parametrize("rows,E,k", [(3000, 100, 17), (15000, 512, 24), (20000, 40, 32)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_route_more_than_16_of_many_rows(cuda_pkg, rows, E, k, dtype):
+    g = _gen(rows + k)
+    logits = _randn(g, rows, E, std=1.5).to(dtype)
+    bias = _randn(g, E, std=0.02)
+    for scoring in ("softmax", "sigmoid"):
+        _check_route(cuda_pkg, logits, k, scoring)
+        _check_route(cuda_pkg, logits, k, scoring, bias=bias)
+        _check_route(cuda_pkg, logits, k, scoring, bias=bias, groups=4, top_groups=4, group_top=2, renorm=False)
