@@ -12,7 +12,7 @@
 // Without bias and with one value per group the logits themselves order the
 // experts, exactly.  Otherwise the values are computed in fp32 first; when two
 // values whose order matters lie closer than the bound on their rounding error
-// the warp decides the row again in fp64 (well under 1% of rows).
+// the warp decides the row again in fp64.
 //
 // Plan: a stable counting sort of the (row, j) pairs by expert, in (row, j)
 // order inside an expert.  Each CTA of the router owns a chunk of rows and
@@ -162,7 +162,15 @@ __device__ __forceinline__ unsigned warp_best(unsigned long long& key, unsigned 
   return at;
 }
 
+// The same of floats.
+__device__ __forceinline__ unsigned float_order(float x) {
+  const int b = __float_as_int(x + 0.0f);
+  return (unsigned)(b ^ ((b >> 31) | (int)0x80000000));
+}
+
 // A row's choices in fp64, a warp to the row.  m: the row's greatest logit or 0.
+// Scores that are equal in fp64 too (sigmoids of 37 and more, exponentials that
+// underflow) follow their logits, as they do without a bias.
 template <typename T>
 __device__ __noinline__ void route_row_exact(const RouteParams& p, const float* bias, const T* lg, float m, int lane,
                                              uint16_t* chosen) {
@@ -221,17 +229,28 @@ __device__ __noinline__ void route_row_exact(const RouteParams& p, const float* 
     for (int i = 0; i < n; ++i)
       if (!((kept >> (((i * 32 + lane) / per) & 31)) & 1u)) v[i] = 0ull;
   }
+  // neither closed nor infinite (by its bias: equal, whatever the score)
+  auto finite = [](unsigned long long k) { return k != 0 && k != 0xfff0000000000000ull; };
 #pragma unroll 1
   for (int j = 0; j < p.top_k; ++j) {
     unsigned long long best = 0;
     unsigned e = lane;
 #pragma unroll 1
-    for (int i = 0; i < n; ++i)
-      if (v[i] > best) {
+    for (int i = 0; i < n; ++i) {
+      const unsigned f = (unsigned)(i * 32 + lane);
+      if (v[i] > best || (v[i] == best && finite(best) && route_load(lg + f) > route_load(lg + e))) {
         best = v[i];
-        e = (unsigned)(i * 32 + lane);
+        e = f;
       }
-    const unsigned at = warp_best(best, e);
+    }
+    unsigned long long top = best;
+    unsigned at = warp_best(top, e);
+    const bool tied = best == top && finite(top);
+    if (__popc(__ballot_sync(0xffffffffu, tied)) > 1) {
+      const unsigned x = tied ? float_order(route_load(lg + e)) : 0u;
+      const unsigned most = __reduce_max_sync(0xffffffffu, x);
+      at = __reduce_min_sync(0xffffffffu, tied && x == most ? e : kNoIndex);
+    }
     if (at != kNoIndex && (at & 31u) == (unsigned)lane) v[at >> 5] = 0ull;
     if (lane == 0) chosen[j] = at != kNoIndex ? (uint16_t)at : kNoChoice;
   }

@@ -907,3 +907,31 @@ def test_route_more_than_16_of_many_rows(cuda_pkg, rows, E, k, dtype):
         _check_route(cuda_pkg, logits, k, scoring)
         _check_route(cuda_pkg, logits, k, scoring, bias=bias)
         _check_route(cuda_pkg, logits, k, scoring, bias=bias, groups=4, top_groups=4, group_top=2, renorm=False)
+
+
+@pytest.mark.parametrize("rows,E,k", [(1, 8, 3), (300, 40, 6), (16000, 96, 8), (5000, 200, 17)])
+def test_route_scores_that_saturate(cuda_pkg, rows, E, k):
+    """Scores whose 64-bit values are equal: the greater logit is the greater score,
+    with a bias of zeros as without a bias, and equal logits go by index."""
+    g = _gen(rows + E)
+    zeros = torch.zeros(E, device=DEV)
+    near = torch.randint(40, 60, (rows, E), generator=g, device=DEV).float()  # sigmoid 1 - 4e-18 and nearer to 1
+    far = torch.randint(-990, -960, (rows, E), generator=g, device=DEV).float()  # exp 0 beside a logit of 0
+    far[:, E - 1] = 0.0
+    for logits, scoring in ((near, "sigmoid"), (far, "softmax"), (far, "sigmoid")):
+        want = cuda_pkg.kernels.route_experts(logits, k, scoring=scoring)
+        order = np.argsort(-logits.cpu().numpy(), axis=1, kind="stable")[:, :k]
+        assert np.array_equal(want.experts.cpu().numpy(), order)
+        got = cuda_pkg.kernels.route_experts(logits, k, scoring=scoring, bias=zeros)
+        assert torch.equal(got.experts, want.experts)
+        got = cuda_pkg.kernels.route_experts(logits, k, scoring=scoring, bias=zeros + 0.25)
+        assert torch.equal(got.experts, want.experts)
+    # a bias decides before a logit does; infinite ones are equal, in index order
+    bias = zeros.clone()
+    bias[1::2] = 1e-6
+    got = cuda_pkg.kernels.route_experts(near, k, scoring="sigmoid", bias=bias).experts.cpu().numpy()
+    odd = np.where(np.arange(E)[None] % 2 == 1, near.cpu().numpy(), near.cpu().numpy() - 100.0)
+    assert np.array_equal(got, np.argsort(-odd, axis=1, kind="stable")[:, :k])
+    bias[2:5] = math.inf
+    got = cuda_pkg.kernels.route_experts(near, 3, scoring="sigmoid", bias=bias).experts
+    assert (got == torch.tensor([2, 3, 4], device=DEV)).all()
