@@ -9,10 +9,10 @@
 // sum 1 if asked, times weight_scale.
 //
 // A choice is a comparison, so it must not depend on how a score was rounded.
-// Without bias and with one value per group the logits themselves order the
-// experts, exactly.  Otherwise the values are computed in fp32 first; when two
-// values whose order matters lie closer than the bound on their rounding error
-// the warp decides the row again in fp64.
+// Without bias the logits themselves order the experts, exactly.  Otherwise the
+// values are computed in fp32 first; when two values (or groups' strengths)
+// whose order matters lie closer than the bound on their own rounding errors the
+// warp decides the row again in fp64.
 //
 // Plan: a stable counting sort of the (row, j) pairs by expert, in (row, j)
 // order inside an expert.  Each CTA of the router owns a chunk of rows and
@@ -131,10 +131,11 @@ __device__ __forceinline__ void row_top2(V& a, V& b, int L) {
     push_top2(a, b, d);
   }
 }
-// A group's strength; -inf without an open expert.
-template <typename V>
-__device__ __forceinline__ V group_strength(V a, V b, int group_top) {
-  return group_top == 2 && b > neg_inf<V>() ? a + b : a;
+// A group's strength (of two values: half their sum, which does not overflow);
+// -inf without an open expert.
+__device__ __forceinline__ float group_strength(float a, float b, int group_top) {
+  if (group_top != 2) return a;
+  return 0.5f * a + (b > neg_inf<float>() ? 0.5f * b : 0.f);
 }
 
 template <typename T>
@@ -187,14 +188,21 @@ __device__ __noinline__ void route_row_exact(const RouteParams& p, const float* 
     }
     z = row_sum(z, 32);
   }
+  bool blunt = false;  // another logit may have an equal value
 #pragma unroll 1
   for (int i = 0; i < n; ++i) {
     const int e = i * 32 + lane;
     const double x = e < p.E ? (double)route_load(lg + e) : neg_inf<double>();
     const double a = exp(p.sigmoid ? -x : x - (double)m);
-    const double w = (p.sigmoid ? 1.0 / (1.0 + a) : a / z) + (double)(p.bias && e < p.E ? bias[e] : 0.f);
-    v[i] = x > neg_inf<double>() && w > neg_inf<double>() ? double_order(w) : 0ull;
+    const double sc = p.sigmoid ? 1.0 / (1.0 + a) : a / z;
+    const double w = sc + (double)(p.bias && e < p.E ? bias[e] : 0.f);
+    const bool in = x > neg_inf<double>() && w > neg_inf<double>();
+    v[i] = in ? double_order(w) : 0ull;
+    // The next fp32 logit is |x| 2^-24 away at least, the next value |w| 2^-52.
+    const float s = (float)sc;
+    blunt |= in && !((p.sigmoid ? s * (1.f - s) : s) * fabsf((float)x) > 1e-6f * fabsf((float)w));
   }
+  blunt = __any_sync(0xffffffffu, blunt);
   if (p.groups > 1) {
     const int per = p.E / p.groups;
     double strength = neg_inf<double>();  // of group `lane`
@@ -228,6 +236,23 @@ __device__ __noinline__ void route_row_exact(const RouteParams& p, const float* 
 #pragma unroll 1
     for (int i = 0; i < n; ++i)
       if (!((kept >> (((i * 32 + lane) / per) & 31)) & 1u)) v[i] = 0ull;
+  }
+  if (!blunt) {
+#pragma unroll 1
+    for (int j = 0; j < p.top_k; ++j) {
+      unsigned long long best = 0;
+      unsigned e = lane;
+#pragma unroll 1
+      for (int i = 0; i < n; ++i)
+        if (v[i] > best) {
+          best = v[i];
+          e = (unsigned)(i * 32 + lane);
+        }
+      const unsigned at = warp_best(best, e);
+      if (at != kNoIndex && (at & 31u) == (unsigned)lane) v[at >> 5] = 0ull;
+      if (lane == 0) chosen[j] = at != kNoIndex ? (uint16_t)at : kNoChoice;
+    }
+    return;
   }
   // neither closed nor infinite (by its bias: equal, whatever the score)
   auto finite = [](unsigned long long k) { return k != 0 && k != 0xfff0000000000000ull; };
@@ -298,12 +323,24 @@ struct RouteList {
   }
 };
 
+// What the bias adds to the choice: without one, scores are ordered like logits.
+struct RouteBias {
+  bool orders;  // the values' order is not that of the logits
+  float most;   // greatest finite value above 0
+};
+
+// Whether two fp32 values a >= b may lie the other way round: each is off by the
+// score's error and its own rounding (infinite ones are exact).
+__device__ __forceinline__ bool too_near(float a, float b, float twice_err) {
+  return a - b < twice_err + 6.1e-8f * (fabsf(a) + fabsf(b));
+}
+
 // One tile: rows [t0, t0 + n) in shared memory, xs[e * pitch + row]; flags[row]
 // set for a row whose scores are not numbers.  Thread = (row, lane of L).
 // Writes the choices to chosen[row * top_k + j] and, by the row's lane 0,
 // top[row], zs[row] for the weights.  All threads of a warp take part.
 template <int KL, typename T>
-__device__ void route_choose(const RouteParams& p, const float* bias, float bias_max, float* xs, int pitch,
+__device__ void route_choose(const RouteParams& p, const float* bias, const RouteBias& rb, float* xs, int pitch,
                              const int* flags, float* strengths, float* tops, float* zs, uint16_t* maybe,
                              uint16_t* chosen, int t0, int n, int L) {
   const int row = (int)threadIdx.x / L, sub = (int)threadIdx.x & (L - 1), lane = (int)threadIdx.x & 31;
@@ -311,7 +348,8 @@ __device__ void route_choose(const RouteParams& p, const float* bias, float bias
   const int E = p.E;
   float* x = xs + (on ? row : 0);
   const bool bad = on && flags[row] != 0;
-  const bool by_value = p.bias != nullptr || (p.groups > 1 && p.group_top == 2);
+  // of one of them the values are needed: to choose experts, or groups by two
+  const bool by_value = rb.orders || (p.groups > 1 && p.group_top == 2);
   float top = 0.f, z = 1.f;
   if (!p.sigmoid && (by_value || !p.renorm)) {
     float m = neg_inf<float>();
@@ -322,33 +360,36 @@ __device__ void route_choose(const RouteParams& p, const float* bias, float bias
     // Blocks of 16 in four parts: one after the other a lane's up to 193 terms
     // could all round the same way, 1.1e-5 of the sum.
     z = 0.f;
-    for (int e0 = sub; e0 < E; e0 += 16 * L) {
+    int e = sub;
+#pragma unroll 1
+    for (; e + 15 * L < E; e += 16 * L) {
       float part[4] = {};
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int e = e0 + i * L;
-        if (e < E) part[i & 3] += expf(x[e * pitch] - top);
-      }
+      for (int i = 0; i < 16; ++i) part[i & 3] += expf(x[(e + i * L) * pitch] - top);
       z += (part[0] + part[1]) + (part[2] + part[3]);
     }
-    z = row_sum(z, L);
+    float rest = 0.f;
+#pragma unroll 1
+    for (; e < E; e += L) rest += expf(x[e * pitch] - top);
+    z = row_sum(z + rest, L);
   }
   const float zi = 1.f / z;
-  float err = -1.f;  // the logits themselves: no two are too close
-  if (by_value && !bad) {
-    // |error of v| <= |error of s| + 2^-24 |v|.  Sigmoid: e = 2^(-x log2 e) with
+  float err = 0.f, group_err = 0.f;
+  if (by_value) {
+    // |error of v| <= |error of s| + 2^-24 |v|; here that of s.  Sigmoid: e = 2^(-x log2 e) with
     // the product rounded (|x| 2^-23 relative) and ex2 within 2 ulp, 1 + e rounded,
     // the quotient within 2 ulp: s (1 - s) (2^-22 + |x| 2^-23) + s (2^-24 + 2^-22),
     // at most 4.2e-7.  Softmax, in 2^-24 of the greatest score, 1 / z: the sum of
-    // n = E / L terms to a lane 5 (a block of 16) + n / 16 + 1 (blocks) + 5 (lanes);
+    // n = E / L terms to a lane 15 (a block, or what fills none) + n / 16 + 1 + 5 (lanes);
     // expf within 2 ulp 4, in the sum and in the score; x - top rounded, d 2^-24
     // of exp(-d): log E <= 6.3 in the sum, 0.4 in the score; 1 / z and the product 2.
     const float smax = p.sigmoid ? 1.f : zi;
-    const float terms = 28.f + 0.0625f * (float)(E / L + 1);
-    err = (p.sigmoid ? 4.2e-7f : 6e-8f * terms * smax) + 6e-8f * (smax + bias_max);
+    const float terms = 39.f + 0.0625f * (float)(E / L + 1);
+    err = p.sigmoid ? 4.2e-7f : 6e-8f * terms * smax;
+    group_err = 2.f * err + 1.3e-7f * (smax + rb.most);
   }
-  // Value of expert e, in place of its logit.
-  const bool set = by_value && on && !bad;
+  // Value of expert e, in place of its logit if values choose.
+  const bool set = rb.orders && on && !bad;
   auto value = [&](int e) {
     const float a = x[e * pitch];
     if (!by_value) return a;
@@ -359,7 +400,7 @@ __device__ void route_choose(const RouteParams& p, const float* bias, float bias
     if (set) x[e * pitch] = v;
     return v;
   };
-  bool close = false;
+  bool close = false, groups_close = false;
   uint32_t kept = 0xffffffffu;
   const int per = E / p.groups;
   if (p.groups > 1) {
@@ -396,9 +437,14 @@ __device__ void route_choose(const RouteParams& p, const float* bias, float bias
     if (!on) kept = 0;
     weakest = -row_max(-weakest, L);
     dropped = row_max(dropped, L);
-    // a strength is a rounded sum of up to two values
-    close = dropped > neg_inf<float>() && weakest - dropped <= 6 * err;
+    // A strength s is (a + b) / 2, rounded, of two values with |a| + |b| <=
+    // 2 |s| + 2 max(a, 0), and a <= the greatest score + bias: off by err + 2^-24
+    // (2 |s| + the greatest).
+    groups_close = by_value && !bad && dropped > neg_inf<float>() &&
+                   weakest - dropped < group_err + 1.3e-7f * (fabsf(weakest) + fabsf(dropped));
   }
+  // (a < -inf is never true)
+  const float twice_err = set ? 2.f * err : neg_inf<float>();
   RouteList<KL> list;
   list.clear();
   if (p.groups > 1) {
@@ -450,7 +496,7 @@ __device__ void route_choose(const RouteParams& p, const float* bias, float bias
     for (int j = 0; j < KL; ++j)
       if (j < p.top_k) {
         const bool found = list.v[j] > neg_inf<float>();
-        close |= found && before - list.v[j] <= 2 * err;  // inf - inf compares false
+        close |= found && too_near(before, list.v[j], twice_err);
         before = list.v[j];
         if (on) out[j] = found ? (uint16_t)list.e[j] : kNoChoice;
       } else {
@@ -462,24 +508,26 @@ __device__ void route_choose(const RouteParams& p, const float* bias, float bias
       int e = list.e[0];
       row_best(v, e, L);
       const bool found = v > neg_inf<float>();
-      close |= found && before - v <= 2 * err;
+      close |= found && too_near(before, v, twice_err);
       before = v;
       if (found && (e & (L - 1)) == sub) list.pop();
       if (on && sub == 0) out[j] = found ? (uint16_t)e : kNoChoice;
     }
     list.rest = row_max(fmaxf(list.rest, list.v[0]), L);
   }
-  close |= list.rest > neg_inf<float>() && before - list.rest <= 2 * err;
+  close |= list.rest > neg_inf<float>() && too_near(before, list.rest, twice_err);
   if (on && sub == 0) {
     tops[row] = top;
     zs[row] = z;
   }
   __syncwarp();
   // Rows too close to call in fp32, the whole warp at each.
-  for (unsigned again = __ballot_sync(0xffffffffu, close && on && sub == 0); again != 0; again &= again - 1) {
-    const int r = ((int)threadIdx.x - lane + __ffs(again) - 1) / L;
-    route_row_exact<T>(p, bias, static_cast<const T*>(p.logits) + (int64_t)(t0 + r) * E, tops[r], lane,
-                       chosen + r * p.top_k);
+  for (unsigned again = __ballot_sync(0xffffffffu, (close || groups_close) && on && sub == 0); again != 0;
+       again &= again - 1) {
+    const int from = __ffs(again) - 1;
+    const int r = ((int)threadIdx.x - lane + from) / L;
+    const T* lg = static_cast<const T*>(p.logits) + (int64_t)(t0 + r) * E;
+    route_row_exact<T>(p, bias, lg, tops[r], lane, chosen + r * p.top_k);
   }
   __syncwarp();
 }
@@ -665,17 +713,18 @@ __global__ void __launch_bounds__(KL > 16 ? 512 : kRouteThreads) route_kernel(co
     float* tops = reinterpret_cast<float*>(flags + p.tile_rows);
     float* zs = tops + p.tile_rows;
     uint16_t* maybe = reinterpret_cast<uint16_t*>(zs + p.tile_rows);  // [kMaybe][threads], with 16 experts a lane
-    float bias_max = 0.f;
-    if (p.bias) {
-      for (int i = threadIdx.x; i < p.E; i += (int)blockDim.x) {
-        const float b = __ldg(p.bias + i);
-        bias[i] = isnan(b) ? neg_inf<float>() : b;  // closed by its bias
+    __shared__ RouteBias rb;
+    if (warp == 0) {
+      float most = 0.f;
+      if (p.bias) {
+        for (int i = lane; i < p.E; i += 32) {
+          const float b = __ldg(p.bias + i);
+          bias[i] = isnan(b) ? neg_inf<float>() : b;  // closed by its bias
+          if (b < -neg_inf<float>()) most = fmaxf(most, b);
+        }
+        most = row_max(most, 32);
       }
-      for (int i = lane; i < p.E; i += 32) {
-        const float b = fabsf(__ldg(p.bias + i));
-        if (b < -neg_inf<float>()) bias_max = fmaxf(bias_max, b);
-      }
-      bias_max = row_max(bias_max, 32);
+      if (lane == 0) rb = {p.bias != nullptr, most};
     }
     for (int t0 = r0; t0 < r1; t0 += p.tile_rows) {
       const int n = min(p.tile_rows, r1 - t0);
@@ -733,7 +782,7 @@ __global__ void __launch_bounds__(KL > 16 ? 512 : kRouteThreads) route_kernel(co
       else
         stage(std::integral_constant<int, 1>());
       __syncthreads();
-      route_choose<KL, T>(p, bias, bias_max, xs, p.pitch, flags, strengths, tops, zs, maybe, chosen, t0, n, p.lanes);
+      route_choose<KL, T>(p, bias, rb, xs, p.pitch, flags, strengths, tops, zs, maybe, chosen, t0, n, p.lanes);
       __syncthreads();
       // the values are done with: the weights take their place on the way out
       route_weights<KL, T>(p, flags, tops, zs, chosen, xs, t0, n, live, p.lanes);

@@ -935,3 +935,47 @@ def test_route_scores_that_saturate(cuda_pkg, rows, E, k):
     bias[2:5] = math.inf
     got = cuda_pkg.kernels.route_experts(near, 3, scoring="sigmoid", bias=bias).experts
     assert (got == torch.tensor([2, 3, 4], device=DEV)).all()
+
+
+def _fastest(fn, n=10):
+    """Least time of n calls on the GPU, in us."""
+    times = []
+    for i in range(n + 2):
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        fn()
+        end.record()
+        torch.cuda.synchronize()
+        times.append(start.elapsed_time(end) * 1e3)
+    return min(times[2:])
+
+
+@pytest.mark.parametrize("groups", [1, 8])
+def test_route_of_an_expert_disabled_by_its_bias(cuda_pkg, groups):
+    """A bias of -1e9 (or the type's lowest) orders like -inf, and costs no more:
+    only values that lie near each other are decided again in 64 bits."""
+    cuda_pkg._lib.set_sync_check(False)
+    k = cuda_pkg.kernels
+    g = _gen(31)
+    logits = _randn(g, 60000, 64, std=1.5)
+    kw = dict(scoring="sigmoid", num_groups=groups, top_groups=min(groups, 3), group_score_top=2)
+    names = dict(groups=groups, top_groups=min(groups, 3), group_top=2)
+    times = []
+    for low in (-math.inf, -1e9, torch.finfo(torch.float32).min):
+        bias = _randn(_gen(32), 64, std=0.05)
+        bias[[3, 40, 41, 42, 43, 44, 45, 46]] = low  # of one group, all but one
+        r = _check_route(cuda_pkg, logits, 6, "sigmoid", bias=bias, **names)
+        if low == -math.inf:
+            want = r.experts
+        assert torch.equal(r.experts, want)
+        times.append(_fastest(lambda: k.route_experts(logits, 6, bias=bias, **kw)))
+    assert max(times) < 1.5 * times[0], times
+    # more choices than experts left: the disabled ones follow, by logit
+    few = _randn(g, 500, 16)
+    bias = torch.full((16,), torch.finfo(torch.float32).min, device=DEV)
+    bias[5] = bias[9] = 0.01
+    for gr in (1, 4):
+        got = k.route_experts(few, 8, scoring="sigmoid", bias=bias, num_groups=gr, top_groups=gr, group_score_top=2).experts
+        first = few.clone()
+        first[:, [5, 9]] += 1e4
+        assert torch.equal(got.long(), first.sort(stable=True, dim=1, descending=True)[1][:, :8])
