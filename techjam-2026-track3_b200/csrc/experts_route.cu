@@ -9,10 +9,12 @@
 // sum 1 if asked, times weight_scale.
 //
 // A choice is a comparison, so it must not depend on how a score was rounded.
-// Without bias the logits themselves order the experts, exactly.  Otherwise the
-// values are computed in fp32 first; when two values (or groups' strengths)
-// whose order matters lie closer than the bound on their own rounding errors the
-// warp decides the row again in fp64.
+// Without a bias, or with the same one for all, the logits themselves order the
+// experts, exactly.  Otherwise the values are computed in fp32 first; when two
+// values whose order matters lie closer than the bound on their rounding errors
+// and their experts' biases differ, or two groups' strengths do, the warp decides
+// the row again in fp64.  Sigmoid, by a restatement: 2 rows in 10^4 (64 experts in
+// groups, fp32 logits) to 8 (256, bf16), 38 under biases of a few fixed steps.
 //
 // Plan: a stable counting sort of the (row, j) pairs by expert, in (row, j)
 // order inside an expert.  Each CTA of the router owns a chunk of rows and
@@ -323,7 +325,8 @@ struct RouteList {
   }
 };
 
-// What the bias adds to the choice: without one, scores are ordered like logits.
+// What the bias adds to the choice: nothing without one or where it is one finite
+// value for all experts (as it starts), since scores are ordered like logits.
 struct RouteBias {
   bool orders;  // the values' order is not that of the logits
   float most;   // greatest finite value above 0
@@ -333,6 +336,43 @@ struct RouteBias {
 // score's error and its own rounding (infinite ones are exact).
 __device__ __forceinline__ bool too_near(float a, float b, float twice_err) {
   return a - b < twice_err + 6.1e-8f * (fabsf(a) + fabsf(b));
+}
+
+// Whether the order of a row's choices is certain although fp32 values lie too
+// near: of two experts with the same bias, the logits decide.  A warp to the row
+// (x: its values); logits in 16 bits are often equal, and biases that were moved
+// by fixed steps too.
+template <typename T>
+__device__ __noinline__ bool route_row_settled(const RouteParams& p, const float* bias, const float* x, int pitch,
+                                               const T* lg, const uint16_t* chosen, uint32_t kept, float twice_err,
+                                               int lane) {
+  // lane j: the j-th choice and the one before it
+  const unsigned e = lane < p.top_k ? chosen[lane] : kNoChoice;
+  const bool in = e != kNoChoice;
+  const float v = in ? x[e * pitch] : 0.f, b = in ? bias[e] : 0.f;
+  const float pv = __shfl_up_sync(0xffffffffu, v, 1), pb = __shfl_up_sync(0xffffffffu, b, 1);
+  const unsigned pe = __shfl_up_sync(0xffffffffu, e, 1);
+  const bool near = lane > 0 && in && too_near(pv, v, twice_err);
+  if (__any_sync(0xffffffffu, near && b != pb)) return false;
+  auto in_order = [&](unsigned e0, unsigned e1) {
+    const float l0 = route_load(lg + e0), l1 = route_load(lg + e1);
+    return l0 > l1 || (l0 == l1 && e0 < e1);
+  };
+  bool open = near && !in_order(pe, e);
+  // the last choice against the experts not chosen
+  const unsigned le = __shfl_sync(0xffffffffu, e, p.top_k - 1);
+  const float lv = __shfl_sync(0xffffffffu, v, p.top_k - 1), lb = __shfl_sync(0xffffffffu, b, p.top_k - 1);
+  if (le != kNoChoice) {
+    const int per = p.E / p.groups;
+#pragma unroll 1
+    for (unsigned f = lane; f < (unsigned)p.E; f += 32) {
+      const float w = x[f * pitch];
+      if (w > neg_inf<float>() && (w < lv || (w == lv && f > le)) && too_near(lv, w, twice_err) &&
+          (p.groups == 1 || ((kept >> (f / per)) & 1u)))
+        open |= bias[f] != lb || !in_order(le, f);
+    }
+  }
+  return !__any_sync(0xffffffffu, open);
 }
 
 // One tile: rows [t0, t0 + n) in shared memory, xs[e * pitch + row]; flags[row]
@@ -435,6 +475,7 @@ __device__ void route_choose(const RouteParams& p, const float* bias, const Rout
     // Threads past the tile's rows follow along on row 0, whose strengths another
     // warp may be writing: they keep no group.
     if (!on) kept = 0;
+    if (on && sub == 0) st[0] = __uint_as_float(kept);  // all lanes of the row have read the strengths
     weakest = -row_max(-weakest, L);
     dropped = row_max(dropped, L);
     // A strength s is (a + b) / 2, rounded, of two values with |a| + |b| <=
@@ -527,6 +568,11 @@ __device__ void route_choose(const RouteParams& p, const float* bias, const Rout
     const int from = __ffs(again) - 1;
     const int r = ((int)threadIdx.x - lane + from) / L;
     const T* lg = static_cast<const T*>(p.logits) + (int64_t)(t0 + r) * E;
+    const float row_err = __shfl_sync(0xffffffffu, twice_err, from);
+    const uint32_t row_kept = p.groups > 1 ? __float_as_uint(strengths[r]) : 0u;
+    if (!__shfl_sync(0xffffffffu, (int)groups_close, from) &&
+        route_row_settled<T>(p, bias, xs + r, pitch, lg, chosen + r * p.top_k, row_kept, row_err, lane))
+      continue;
     route_row_exact<T>(p, bias, lg, tops[r], lane, chosen + r * p.top_k);
   }
   __syncwarp();
@@ -715,16 +761,20 @@ __global__ void __launch_bounds__(KL > 16 ? 512 : kRouteThreads) route_kernel(co
     uint16_t* maybe = reinterpret_cast<uint16_t*>(zs + p.tile_rows);  // [kMaybe][threads], with 16 experts a lane
     __shared__ RouteBias rb;
     if (warp == 0) {
+      bool orders = false;
       float most = 0.f;
       if (p.bias) {
+        const float first = __ldg(p.bias);
         for (int i = lane; i < p.E; i += 32) {
           const float b = __ldg(p.bias + i);
           bias[i] = isnan(b) ? neg_inf<float>() : b;  // closed by its bias
+          orders |= b != first;                       // NaN, too
           if (b < -neg_inf<float>()) most = fmaxf(most, b);
         }
+        orders = __any_sync(0xffffffffu, orders) || isinf(first);
         most = row_max(most, 32);
       }
-      if (lane == 0) rb = {p.bias != nullptr, most};
+      if (lane == 0) rb = {orders, most};
     }
     for (int t0 = r0; t0 < r1; t0 += p.tile_rows) {
       const int n = min(p.tile_rows, r1 - t0);

@@ -979,3 +979,25 @@ def test_route_of_an_expert_disabled_by_its_bias(cuda_pkg, groups):
         first = few.clone()
         first[:, [5, 9]] += 1e4
         assert torch.equal(got.long(), first.sort(stable=True, dim=1, descending=True)[1][:, :8])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("groups", [1, 8])
+def test_route_of_equal_values(cuda_pkg, dtype, groups):
+    """16-bit logits under a bias of zeros, of one value and of a few steps: the
+    order is that of the logits inside each bias, at the cost of any other."""
+    cuda_pkg._lib.set_sync_check(False)
+    k = cuda_pkg.kernels
+    g = _gen(33)
+    logits = _randn(g, 30000, 256, std=1.5).to(dtype)
+    names = dict(groups=groups, top_groups=min(groups, 4), group_top=1)
+    kw = dict(scoring="sigmoid", num_groups=groups, top_groups=min(groups, 4), group_score_top=1)
+    spread = _randn(g, 256, std=0.05)
+    any_other = _fastest(lambda: k.route_experts(logits, 8, bias=spread, **kw))
+    for bias in (torch.zeros(256, device=DEV), torch.full((256,), 0.3, device=DEV),
+                 torch.randint(-3, 4, (256,), generator=g, device=DEV) * 0.001, spread):
+        for scoring in ("sigmoid", "softmax"):
+            _check_route(cuda_pkg, logits, 8, scoring, bias=bias, **names)
+        assert _fastest(lambda: k.route_experts(logits, 8, bias=bias, **kw)) < 1.5 * any_other
+    _check_route(cuda_pkg, logits, 8, "sigmoid", bias=spread, **(names | dict(group_top=2)))
+    _check_route(cuda_pkg, logits, 8, "softmax", **(names | dict(group_top=2)))
