@@ -619,6 +619,7 @@ def expert_ffn(a, w_in, b_in, w_out, b_out, routing, *, out=None):
     _no_grad(a, w_in, b_in, w_out, b_out)
     code = _half_dtype(a, "a")
     _require_routing(routing, dev)
+    _no_grad(routing.weights)
     E = routing.num_experts
     if a.dim() != 2 or a.shape[0] != routing.rows:
         raise ValueError(f"a must be [{routing.rows}, D], got {tuple(a.shape)}")

@@ -205,3 +205,18 @@ def test_routing_buffers_are_checked(k, experts, weights, plan, error):
     k.ExpertRouting(torch.zeros(4, 2, dtype=I32), torch.zeros(4, 2), torch.zeros(20, dtype=I32), 3)
     with pytest.raises(error):
         k.ExpertRouting(experts, weights, plan, 3)
+
+
+def test_weights_of_the_routing_that_need_a_gradient_are_refused(k):
+    """A routing may be made of weights that need one; whatever sums with them refuses."""
+    r = k.ExpertRouting(torch.zeros(4, 2, dtype=I32), torch.zeros(4, 2, requires_grad=True),
+                        torch.zeros(4 + 24, dtype=I32), 3)
+    a, y = torch.zeros(4, 16, dtype=F16), torch.zeros(8, 16, dtype=F16)
+    w_in, w_out = torch.zeros(3, 32, 16, dtype=F16), torch.zeros(3, 16, 32, dtype=F16)
+    calls = (lambda: k.expert_ffn(a, w_in, None, w_out, None, r), lambda: k.expert_combine(y, r),
+             lambda: k.sandwich_norm(torch.zeros(4, 16), y, torch.ones(16), routing=r))
+    for call in calls:
+        with pytest.raises(RuntimeError, match="autograd"):
+            call()
+        with torch.no_grad(), pytest.raises(_Unreached):
+            call()
