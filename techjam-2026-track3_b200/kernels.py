@@ -14,6 +14,7 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -368,7 +369,12 @@ _GATES = {"none": _lib.TJ_GATE_NONE, "sigmoid": _lib.TJ_GATE_SIGMOID, "tanh": _l
 
 
 def _no_grad(*tensors) -> None:
-    """Forward only, like the encoder: a call whose gradient would be lost raises."""
+    """Forward only, like the encoder: a call whose gradient (or forward-mode
+    tangent, which no_grad does not switch off) would be lost raises."""
+    if forward_ad._current_level >= 0:  # inside a dual_level
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("forward-mode autograd through this operator is not supported")
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:

@@ -220,3 +220,30 @@ def test_weights_of_the_routing_that_need_a_gradient_are_refused(k):
             call()
         with torch.no_grad(), pytest.raises(_Unreached):
             call()
+
+
+def test_forward_mode_tangents_are_refused(k):
+    from torch.autograd import forward_ad
+
+    def dual(*shape, dtype=F32):
+        return forward_ad.make_dual(torch.zeros(*shape, dtype=dtype), torch.ones(*shape, dtype=dtype))
+
+    r = _routing(k)
+    a, y = torch.zeros(4, 16, dtype=F16), torch.zeros(8, 16, dtype=F16)
+    w_in, w_out = torch.zeros(3, 32, 16, dtype=F16), torch.zeros(3, 16, 32, dtype=F16)
+    with forward_ad.dual_level():
+        with pytest.raises(_Unreached):  # no tangent: nothing to lose
+            k.route_experts(torch.zeros(4, 8), 2)
+        calls = (lambda: k.route_experts(dual(4, 8), 2),
+                 lambda: k.route_experts(torch.zeros(4, 8), 2, bias=dual(8)),
+                 lambda: k.expert_plan(torch.zeros(4, 2, dtype=I32), dual(4, 2), 3),
+                 lambda: k.gemm_experts(a, dual(3, 32, 16, dtype=F16), None, r, gather=True),
+                 lambda: k.expert_combine(dual(8, 16, dtype=F16), r),
+                 lambda: k.expert_ffn(dual(4, 16, dtype=F16), w_in, None, w_out, None, r),
+                 lambda: k.sandwich_norm(dual(4, 16), a, torch.ones(16)),
+                 lambda: k.sandwich_norm(torch.zeros(4, 16), y, dual(16), routing=r))
+        for call in calls:
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                call()
