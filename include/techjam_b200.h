@@ -253,7 +253,8 @@ TJ_API int tj_flash_attn_fwd_partial(const void* q16, const void* k16, const voi
  * Layouts: logits [rows, E]; experts int32 and weights float32 [rows, top_k];
  * activations and weights float16 or bfloat16, weights [E, N, K] (nn.Linear
  * layout per expert), biases float32 [E, N].  "Slots" are the (row, j) pairs
- * sorted by expert, in (row, j) order inside an expert.
+ * sorted by expert, in (row, j) order inside an expert.  Outputs and workspaces
+ * share no memory with inputs, but out of tj_expert_ffn may be a.
  */
 #define TJ_DTYPE_F32 0
 #define TJ_DTYPE_F16 1
@@ -351,7 +352,8 @@ TJ_API int tj_expert_ffn(const void* a, int dtype, const void* w_in, const float
  * rows_per_gate >= rows for a gate per channel, rows_per_gate = seq_len for
  * one per sample, 1 for one per row.  d_model up to 32768 (8192 when it is not
  * a multiple of 8 or a pointer is not 16-byte aligned).  sum_out may be x
- * itself when row_map is NULL.  A row map entry or gate row outside its buffer
+ * itself when row_map is NULL, y16 branch16 itself without weights; else outputs
+ * share no memory with inputs.  A row map entry or gate row outside its buffer
  * is recorded as a device error and the row is left out. */
 typedef struct tj_sandwich_desc {
   const float* x;           /* [x_rows, D] */

@@ -411,6 +411,13 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
             and b.data_ptr() < a.data_ptr() + a.numel() * a.element_size())
 
 
+def _require_apart(out: torch.Tensor, name: str, **others) -> None:
+    """out shares no memory with an input that the kernels may read after its first rows are written."""
+    for other, t in others.items():
+        if t is not None and _overlap(out, t):
+            raise ValueError(f"{name} must not share memory with {other}")
+
+
 def _half_dtype(t: torch.Tensor, name: str) -> int:
     if t.dtype not in (torch.float16, torch.bfloat16):
         raise TypeError(f"{name} must be float16 or bfloat16, got {t.dtype}")
@@ -576,8 +583,7 @@ def gemm_experts(a, w, bias, routing, *, gather, gelu=False, out=None):
         out = torch.empty(slots, N, dtype=a.dtype, device=dev)
     else:
         _require_out(out, "out", (slots, N), a.dtype, dev)
-        if _overlap(out, a) or _overlap(out, w):
-            raise ValueError("out must not share memory with a or w")
+        _require_apart(out, "out", a=a, w=w, bias=bias, routing=routing.plan)
     lib = _lib.load()
     need = lib.tj_gemm_experts_workspace_bytes(routing.rows, routing.top_k, routing.num_experts, K, 1 if gather else 0)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
@@ -605,8 +611,7 @@ def expert_combine(y, routing, *, out=None):
         out = torch.empty(routing.rows, D, dtype=y.dtype, device=dev)
     else:
         _require_out(out, "out", (routing.rows, D), y.dtype, dev)
-        if _overlap(out, y):
-            raise ValueError("out must not share memory with y")
+        _require_apart(out, "out", y=y, weights=routing.weights, routing=routing.plan, row_count=routing.row_count)
     rc = _launch(
         dev, _lib.load().tj_expert_combine, y.data_ptr(), code, routing.weights.data_ptr(), routing.plan.data_ptr(),
         _ptr(routing.row_count), routing.rows, routing.top_k, routing.num_experts, D, out.data_ptr(),
@@ -620,7 +625,7 @@ def expert_ffn(a, w_in, b_in, w_out, b_out, routing, *, out=None):
     experts run ffn_in, erf-GELU and ffn_out on it and out is their weighted
     sum.  w_in [E, F, D], w_out [E, D, F], biases [E, F] and [E, D] float32 or
     None, D and F multiples of 8.  Zeros for a row without experts; rows at or
-    past the routing's row_count are left as they were."""
+    past the routing's row_count are left as they were.  out may be a."""
     dev = _cuda_tensor(a, "a")
     _no_grad(a, w_in, b_in, w_out, b_out)
     code = _half_dtype(a, "a")
@@ -640,12 +645,14 @@ def expert_ffn(a, w_in, b_in, w_out, b_out, routing, *, out=None):
         _require_shape(b_in, "b_in", (E, F), torch.float32, dev)
     if b_out is not None:
         _require_shape(b_out, "b_out", (E, D), torch.float32, dev)
-    lib = _lib.load()
     rows, top_k = routing.experts.shape
     if out is None:
         out = torch.empty(rows, D, dtype=a.dtype, device=dev)
     else:
         _require_out(out, "out", (rows, D), a.dtype, dev)
+        _require_apart(out, "out", w_in=w_in, b_in=b_in, w_out=w_out, b_out=b_out, weights=routing.weights,
+                       routing=routing.plan, row_count=routing.row_count)
+    lib = _lib.load()
     need = lib.tj_expert_ffn_workspace_bytes(rows, top_k, E, D, F)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     rc = _launch(
@@ -674,9 +681,9 @@ def sandwich_norm(x, branch, pre_gamma, pre_beta=None, *, post_gamma=None, post_
     row r reading gate row gate_map[r] // rows_per_gate (gate_map: int32,
     default row_map, else r): a sample's gate with rows_per_gate = seq_len, a
     token's with 1.  act: none, sigmoid or tanh.  x [x_rows, D] float32; sum_out
-    may be x when there is no row_map, out branch when there is no routing.  Rows
-    at or past row_count (default:
-    the routing's) are left as they were."""
+    may be x when there is no row_map, out branch when there is no routing, and
+    neither may share memory with another input.  Rows at or past row_count
+    (default: the routing's) are left as they were."""
     dev = _cuda_tensor(x, "x")
     _no_grad(x, branch, pre_gamma, pre_beta, post_gamma, post_beta, gate)
     _require(x, "x", torch.float32, dev)
@@ -738,22 +745,25 @@ def sandwich_norm(x, branch, pre_gamma, pre_beta=None, *, post_gamma=None, post_
                 _require_shape(gate_map, "gate_map", (rows,), torch.int32, dev)
             elif gate_rows * rows_per_gate < rows:
                 raise ValueError(f"gate has {gate_rows} rows of {rows_per_gate} rows each, {rows} rows to gate")
+    # what other rows, or later ones, read
+    read = dict(pre_gamma=pre_gamma, pre_beta=pre_beta, post_gamma=post_gamma, post_beta=post_beta, gate=gate,
+                row_map=row_map, gate_map=gate_map, row_count=row_count)
+    if routing is not None:
+        read.update(weights=routing.weights, routing=routing.plan)
     if sum_out is None:
         sum_out = torch.empty(rows, D, dtype=torch.float32, device=dev)
     else:
         _require_out(sum_out, "sum_out", (rows, D), torch.float32, dev)
         if _overlap(sum_out, x) and (row_map is not None or sum_out.data_ptr() != x.data_ptr()):
             raise ValueError("sum_out may share memory with x only as x itself, without row_map")
-        if _overlap(sum_out, branch):
-            raise ValueError("sum_out must not share memory with branch")
+        _require_apart(sum_out, "sum_out", branch=branch, **read)
     if out is None:
         out = torch.empty(rows, D, dtype=branch.dtype, device=dev)
     else:
         _require_out(out, "out", (rows, D), branch.dtype, dev)
         if _overlap(out, branch) and (routing is not None or out.data_ptr() != branch.data_ptr()):
             raise ValueError("out may share memory with branch only as branch itself, without routing")
-        if _overlap(out, x) or _overlap(out, sum_out):
-            raise ValueError("out must not share memory with x or sum_out")
+        _require_apart(out, "out", x=x, sum_out=sum_out, **read)
     desc = _lib.SandwichDesc(
         x.data_ptr(), _ptr(row_map), branch.data_ptr(), routing.weights.data_ptr() if routing is not None else None,
         routing.row_slot.data_ptr() if routing is not None else None, _ptr(post_gamma), _ptr(post_beta),

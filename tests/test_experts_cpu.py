@@ -247,3 +247,63 @@ def test_forward_mode_tangents_are_refused(k):
                 call()
             with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
                 call()
+
+
+def _views(nbytes):
+    """Views of one buffer: floats [4, 16], halves [4, 16], ints and vectors over the same bytes."""
+    raw = torch.zeros(nbytes, dtype=torch.uint8)
+    return lambda dtype, *shape: raw[: torch.Size(shape).numel() * torch.empty(0, dtype=dtype).element_size()].view(dtype).view(shape)
+
+
+@pytest.mark.parametrize("out", ["sum_out", "out"])
+@pytest.mark.parametrize("name,dtype,shape", [
+    ("gate", F32, (2, 16)), ("gate", F32, (16,)), ("gate", F16, (4, 16)), ("pre_gamma", F32, (16,)), ("pre_beta", F32, (16,)),
+    ("post_gamma", F32, (16,)), ("post_beta", F32, (16,)), ("row_map", I32, (4,)), ("gate_map", I32, (4,)),
+    ("row_count", I32, (1,))])
+def test_sandwich_outputs_over_other_inputs_are_refused(k, out, name, dtype, shape):
+    """Another row's output would be written over what this row still reads."""
+    view = _views(256)
+    args = dict(x=torch.zeros(4, 16), branch=torch.zeros(4, 16, dtype=F16), pre_gamma=torch.ones(16))
+    args[name] = view(dtype, *shape)
+    if name == "post_beta":
+        args["post_gamma"] = torch.ones(16)
+    if name == "gate" and len(shape) == 2:
+        args["rows_per_gate"] = 4 // shape[0]
+    if name == "gate_map":
+        args["gate"] = torch.zeros(4, 16)
+    with pytest.raises(_Unreached):
+        k.sandwich_norm(**args)
+    args[out] = view(F32 if out == "sum_out" else F16, 4, 16)
+    with pytest.raises(ValueError, match="share memory with " + name):
+        k.sandwich_norm(**args)
+
+
+@pytest.mark.parametrize("name", ["weights", "plan", "row_count"])
+def test_outputs_over_the_routing_are_refused(k, name):
+    view = _views(512)
+    parts = dict(experts=torch.zeros(4, 2, dtype=I32), weights=torch.zeros(4, 2), plan=torch.zeros(28, dtype=I32),
+                 row_count=torch.zeros(1, dtype=I32))
+    parts[name] = view(parts[name].dtype, *parts[name].shape)
+    r = k.ExpertRouting(parts["experts"], parts["weights"], parts["plan"], 3, parts["row_count"])
+    a, y, out = torch.zeros(4, 16, dtype=F16), torch.zeros(8, 16, dtype=F16), view(F16, 4, 16)
+    w_in, w_out = torch.zeros(3, 32, 16, dtype=F16), torch.zeros(3, 16, 32, dtype=F16)
+    calls = [lambda: k.expert_combine(y, r, out=out), lambda: k.expert_ffn(a, w_in, None, w_out, None, r, out=out),
+             lambda: k.sandwich_norm(torch.zeros(4, 16), y, torch.ones(16), routing=r, out=out),
+             lambda: k.sandwich_norm(torch.zeros(4, 16), y, torch.ones(16), routing=r, sum_out=view(F32, 4, 16))]
+    if name == "plan":
+        calls.append(lambda: k.gemm_experts(y, w_in[:, :16].contiguous(), None, r, gather=False, out=view(F16, 8, 16)))
+    for call in calls:
+        with pytest.raises(ValueError, match="share"):
+            call()
+
+
+def test_ffn_output_over_weights_is_refused_and_over_a_is_not(k):
+    r = _routing(k)
+    a = torch.zeros(4, 16, dtype=F16)
+    w_in, w_out = torch.zeros(3, 32, 16, dtype=F16), torch.zeros(3, 16, 32, dtype=F16)
+    b_out = torch.zeros(3, 16)
+    with pytest.raises(_Unreached):
+        k.expert_ffn(a, w_in, None, w_out, b_out, r, out=a)
+    for out in (w_in[0, :4], w_out.view(-1)[:64].view(4, 16), b_out.view(F16).view(-1)[:64].view(4, 16)):
+        with pytest.raises(ValueError, match="share"):
+            k.expert_ffn(a, w_in, None, w_out, b_out, r, out=out)
