@@ -396,6 +396,13 @@ def _require_shape(t, name: str, shape, dtype: torch.dtype, device: torch.device
     raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
+def _require_ints(**values) -> None:
+    """The C entries take 32-bit ints, and ctypes would drop the rest without a word."""
+    for name, v in values.items():
+        if not -(2**31) <= v < 2**31:
+            raise ValueError(f"{name} = {v} does not fit 32 bits")
+
+
 def _require_count(row_count, device: torch.device) -> None:
     if row_count is not None:
         _require(row_count, "row_count", torch.int32, device)
@@ -444,6 +451,7 @@ class ExpertRouting:
             raise ValueError(f"experts must be [rows, top_k], got {tuple(self.experts.shape)}")
         dev = self.plan.device
         _require(self.experts, "experts", torch.int32, dev)
+        _require_ints(rows=self.experts.shape[0], num_experts=self.num_experts)
         _require_shape(self.weights, "weights", self.experts.shape, torch.float32, dev)
         _require(self.plan, "plan", torch.int32, dev)
         if self.plan.numel() < self.num_experts + 1 + 2 * self.experts.numel():
@@ -510,6 +518,8 @@ def route_experts(logits, top_k, *, scoring="softmax", bias=None, num_groups=1, 
     if logits.dim() != 2:
         raise ValueError(f"logits must be [rows, experts], got {tuple(logits.shape)}")
     rows, E = logits.shape
+    if rows >= 2**31 or num_groups != 1 or top_groups != 1 or group_score_top != 1:
+        _require_ints(rows=rows, num_groups=num_groups, top_groups=top_groups, group_score_top=group_score_top)
     if scoring not in _SCORES:
         raise ValueError(f"scoring must be one of {sorted(_SCORES)}, got {scoring!r}")
     if not 1 <= top_k <= min(E, 32):
@@ -540,6 +550,7 @@ def expert_plan(experts, weights, num_experts, *, row_count=None) -> ExpertRouti
     if experts.dim() != 2 or not 1 <= experts.shape[1] <= 32:
         raise ValueError(f"experts must be [rows, top_k] with top_k in 1..32, got {tuple(experts.shape)}")
     rows, top_k = experts.shape
+    _require_ints(rows=rows)
     _require_shape(weights, "weights", (rows, top_k), torch.float32, dev)
     _require_count(row_count, dev)
     if not 1 <= num_experts <= 512:
@@ -577,6 +588,8 @@ def gemm_experts(a, w, bias, routing, *, gather, gelu=False, out=None):
     if w.dim() != 3 or w.shape[0] != routing.num_experts or w.shape[2] != K:
         raise ValueError(f"w must be [{routing.num_experts}, N, {K}], got {tuple(w.shape)}")
     N = w.shape[1]
+    if N >= 2**31 or K >= 2**31:
+        _require_ints(N=N, K=K)
     if bias is not None:
         _require_shape(bias, "bias", (routing.num_experts, N), torch.float32, dev)
     if out is None:
@@ -607,6 +620,7 @@ def expert_combine(y, routing, *, out=None):
         raise ValueError(f"y must be a matrix, got {tuple(y.shape)}")
     D = y.shape[1]
     _require_shape(y, "y", (routing.rows * routing.top_k, D), y.dtype, dev)
+    _require_ints(D=D)
     if out is None:
         out = torch.empty(routing.rows, D, dtype=y.dtype, device=dev)
     else:
@@ -640,6 +654,8 @@ def expert_ffn(a, w_in, b_in, w_out, b_out, routing, *, out=None):
     if w_in.dim() != 3 or w_in.shape[0] != E or w_in.shape[2] != D:
         raise ValueError(f"w_in must be [{E}, F, {D}], got {tuple(w_in.shape)}")
     F = w_in.shape[1]
+    if D >= 2**31 or F >= 2**31:
+        _require_ints(D=D, F=F)
     _require_shape(w_out, "w_out", (E, D, F), a.dtype, dev)
     if b_in is not None:
         _require_shape(b_in, "b_in", (E, F), torch.float32, dev)
@@ -708,6 +724,8 @@ def sandwich_norm(x, branch, pre_gamma, pre_beta=None, *, post_gamma=None, post_
             raise ValueError(f"branch must be [rows, {D}], got {tuple(branch.shape)}")
         rows = branch.shape[0]
         _require_shape(branch, "branch", (rows, D), branch.dtype, dev)
+    if rows >= 2**31 or x.shape[0] >= 2**31 or D >= 2**31:
+        _require_ints(rows=rows, x_rows=x.shape[0], columns=D)
     _require_count(row_count, dev)
     if row_map is not None:
         _require_shape(row_map, "row_map", (rows,), torch.int32, dev)
@@ -739,6 +757,7 @@ def sandwich_norm(x, branch, pre_gamma, pre_beta=None, *, post_gamma=None, post_
             if rows_per_gate < 1:
                 raise ValueError(f"rows_per_gate must be at least 1, got {rows_per_gate}")
             gate_rows, gate_code = gate.shape[0], _DTYPES[gate.dtype]
+            _require_ints(gate_rows=gate_rows, rows_per_gate=rows_per_gate)
             if gate_map is None:
                 gate_map = row_map
             if gate_map is not None:

@@ -307,3 +307,33 @@ def test_ffn_output_over_weights_is_refused_and_over_a_is_not(k):
     for out in (w_in[0, :4], w_out.view(-1)[:64].view(4, 16), b_out.view(F16).view(-1)[:64].view(4, 16)):
         with pytest.raises(ValueError, match="share"):
             k.expert_ffn(a, w_in, None, w_out, b_out, r, out=out)
+
+
+def test_sizes_past_32_bits_are_refused(k):
+    """Not taken modulo 2^32: tensors without storage stand for the large ones."""
+    many = 2**32 + 5
+
+    def meta(*shape, dtype=F32):
+        return torch.empty(*shape, dtype=dtype, device="meta")
+
+    r = _routing(k)
+    rm = k.ExpertRouting(meta(4, 2, dtype=I32), meta(4, 2), meta(28, dtype=I32), 3)
+    calls = [lambda kw=kw: k.route_experts(torch.zeros(4, 8), 2, **kw)
+             for kw in (dict(num_groups=2**32 + 2), dict(num_groups=2, top_groups=2**32 + 1),
+                        dict(num_groups=2, group_score_top=2**32 + 1))]
+    calls += [lambda: k.route_experts(meta(many, 1), 1),
+              lambda: k.expert_plan(meta(many, 1, dtype=I32), meta(many, 1), 3),
+              lambda: k.ExpertRouting(meta(many, 1, dtype=I32), meta(many, 1), meta(4 * many, dtype=I32), 3),
+              lambda: k.ExpertRouting(r.experts, r.weights, r.plan, -(2**32) + 3),
+              lambda: k.sandwich_norm(meta(many, 1), meta(many, 1, dtype=F16), meta(1)),
+              lambda: k.sandwich_norm(meta(many, 1), meta(5, 1, dtype=F16), meta(1)),
+              lambda: k.sandwich_norm(torch.zeros(4, 16), torch.zeros(4, 16, dtype=F16), torch.ones(16),
+                                      gate=torch.zeros(1, 16), rows_per_gate=2**32 + 4),
+              lambda: k.gemm_experts(meta(4, many, dtype=F16), meta(3, 8, many, dtype=F16), None, rm, gather=True),
+              lambda: k.gemm_experts(meta(4, 8, dtype=F16), meta(3, many, 8, dtype=F16), None, rm, gather=True),
+              lambda: k.expert_combine(meta(8, many, dtype=F16), rm),
+              lambda: k.expert_ffn(meta(4, 8, dtype=F16), meta(3, many, 8, dtype=F16), None, meta(3, 8, many, dtype=F16), None,
+                                   rm)]
+    for call in calls:
+        with pytest.raises(ValueError, match="32 bits"):
+            call()
