@@ -523,7 +523,8 @@ __global__ void __launch_bounds__(512, 1) sandwich_ring_kernel(const SandwichPar
   uint32_t phase = 0;
   volatile int gave_up = 0;  // of this thread; the team agrees on leaving below
   bool bad = false;
-  for (int64_t row = row0; row < limit; row += step) {
+  int64_t row = row0;
+  for (; row < limit; row += step) {
     const bool ok = mbar_wait(bar_at(stage), phase, &gave_up, 260);
     const RingMeta* meta = reinterpret_cast<const RingMeta*>(stage_at(stage));
     const uint8_t* base = reinterpret_cast<const uint8_t*>(meta) + sizeof(RingMeta);
@@ -634,9 +635,13 @@ __global__ void __launch_bounds__(512, 1) sandwich_ring_kernel(const SandwichPar
     }
   }
   pdl_trigger();
-  // After a wait that ran out, copies may still be on their way into the ring.
+  // After a wait that ran out, copies may still be on their way into the ring:
+  // those of this row and of the up to stages - 1 after it.
   if (k == 0 && bad)
-    for (int s = 0; s < sh.stages; ++s) drain_wait(bar_at(s), s < stage ? phase ^ 1 : phase);
+    for (int s = 0; s < sh.stages; ++s) {
+      const int ahead = s < stage ? s - stage + sh.stages : s - stage;
+      if (row + (int64_t)ahead * step < limit) drain_wait(bar_at(s), s < stage ? phase ^ 1 : phase);
+    }
 }
 
 // Teams and stages for the row's bytes: two stages each while that leaves ten
