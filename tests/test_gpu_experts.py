@@ -1001,3 +1001,106 @@ def test_route_of_equal_values(cuda_pkg, dtype, groups):
         assert _fastest(lambda: k.route_experts(logits, 8, bias=bias, **kw)) < 1.5 * any_other
     _check_route(cuda_pkg, logits, 8, "sigmoid", bias=spread, **(names | dict(group_top=2)))
     _check_route(cuda_pkg, logits, 8, "softmax", **(names | dict(group_top=2)))
+
+
+@pytest.mark.parametrize("rows", [1, 20, 64, 65, 1500])
+def test_expert_ffn_captured_and_on_two_streams(cuda_pkg, rows):
+    """Router and FFN with nothing between their kernels: back to back (FFN-out loads
+    weights before FFN-in has ended, the next call reuses the workspace's memory),
+    captured and replayed on new inputs, and two at once; bit equal to one alone."""
+    cuda_pkg._lib.set_sync_check(False)
+    k = cuda_pkg.kernels
+    g = _gen(rows)
+    E, D, F = 4, 512, 1024  # 32 slots per expert at 64 rows
+    w_in, w_out = _weights(g, E, F, D, torch.float16), _weights(g, E, D, F, torch.float16)
+    b_in, b_out = _randn(g, E, F), _randn(g, E, D)
+    inputs = [(_randn(g, rows, E), _randn(g, rows, D, dtype=torch.float16)) for _ in range(4)]
+
+    def run(logits, a):
+        r = k.route_experts(logits, 2)
+        return k.expert_ffn(a, w_in, b_in, w_out, b_out, r)
+
+    want = []
+    for logits, a in inputs:
+        want.append(run(logits, a))
+        torch.cuda.synchronize()
+    assert not torch.equal(want[0], want[1])
+    outs = [(i, run(*inputs[i])) for _ in range(10) for i in range(4)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want[i]) for i, out in outs)
+    graphs = []
+    for n in (1, 2):  # two graphs, of one call and of two
+        logits, a = inputs[0][0].clone(), inputs[0][1].clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = [run(logits, a) for _ in range(n)]
+        graphs.append((graph, logits, a, got))
+    for i in (1, 2, 3, 0):
+        for graph, logits, a, _ in graphs:
+            logits.copy_(inputs[i][0])
+            a.copy_(inputs[i][1])
+            graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, want[i]) for *_, got in graphs for out in got)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs = []
+    for _ in range(10):
+        for s, i in zip(streams, (1, 2)):
+            with torch.cuda.stream(s):
+                outs.append((i, run(*inputs[i])))
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want[i]) for i, out in outs)
+    assert cuda_pkg._lib.device_status(torch.cuda.current_stream().cuda_stream) == [0, 0, 0, 0]
+
+
+def test_expert_ffn_in_place(cuda_pkg):
+    k = cuda_pkg.kernels
+    for rows in (7, 400):
+        g = _gen(rows)
+        a = _randn(g, rows, 64, dtype=torch.bfloat16)
+        w_in, w_out = _weights(g, 4, 128, 64, torch.bfloat16), _weights(g, 4, 64, 128, torch.bfloat16)
+        r = k.route_experts(_randn(g, rows, 4), 2)
+        want = k.expert_ffn(a, w_in, None, w_out, None, r)
+        assert k.expert_ffn(a, w_in, None, w_out, None, r, out=a) is a and torch.equal(a, want)
+
+
+@pytest.mark.parametrize("rows,D", [(700, 64), (2500, 1021), (900, 4096)])
+def test_sandwich_norm_skips_bad_rows_of_many(cuda_pkg, rows, D):
+    """Map entries, gate rows and slots outside their buffers, spread over teams and
+    stages of the shared-memory path: recorded, those rows left as they were (a
+    bad slot's share left out), all others as without them."""
+    L, k = cuda_pkg._lib, cuda_pkg.kernels
+    L.set_sync_check(False)
+    stream = torch.cuda.current_stream().cuda_stream
+    g = _gen(rows)
+    x, b = _randn(g, rows, D), _randn(g, rows, D, dtype=torch.float16)
+    pg, pb = _affine(g, D)
+    gate = _randn(g, 8, D)
+    per = -(-rows // 8)
+    rm = torch.randperm(rows, generator=g, device=DEV).int()
+    bad = torch.arange(rows, device=DEV) % 7 == 3
+    bad[-1] = bad[0] = True
+    broken = torch.where(bad, torch.where(rm % 2 == 0, rows + 5, -4), rm).int()
+
+    def run(row_map=None, gate_map=None):
+        s, y = torch.full((rows, D), 9.0, device=DEV), torch.full((rows, D), 8.0, dtype=torch.float16, device=DEV)
+        return k.sandwich_norm(x, b, pg, pb, post_gamma=pg, gate=gate, rows_per_gate=per, row_map=row_map,
+                               gate_map=gate_map, sum_out=s, out=y)
+
+    for good, kw in ((run(rm), dict(row_map=broken)), (run(None, rm), dict(gate_map=torch.where(bad, 8 * per, rm).int()))):
+        assert L.device_status(stream) == [0, 0, 0, 0]
+        s, y = run(**kw)
+        with pytest.raises(L.TJError, match="outside"):
+            L.device_status(stream)
+        assert (s[bad] == 9).all() and (y[bad] == 8).all()
+        assert torch.equal(s[~bad], good[0][~bad]) and torch.equal(y[~bad], good[1][~bad])
+    r = k.route_experts(_randn(g, rows, 5), 2)
+    y2 = _randn(g, rows * 2, D, dtype=torch.float16)
+    r.row_slot[bad, 1] = 2 * rows  # one past the branch
+    got = k.sandwich_norm(x, y2, pg, pb, post_gamma=pg, routing=r)
+    with pytest.raises(L.TJError, match="outside"):
+        L.device_status(stream)
+    r.row_slot[bad, 1] = -1
+    want = k.sandwich_norm(x, y2, pg, pb, post_gamma=pg, routing=r)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert L.device_status(stream) == [0, 0, 0, 0]
