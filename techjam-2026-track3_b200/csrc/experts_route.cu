@@ -180,7 +180,6 @@ __device__ __noinline__ void route_row_exact(const RouteParams& p, const float* 
   constexpr int V = kRouteMaxExperts / 32;
   const int n = (p.E + 31) / 32;  // of the V places used
   unsigned long long v[V];        // of experts i * 32 + lane
-  double score[V];
   double z = 1.0;
   if (!p.sigmoid) {
     z = 0.0;
@@ -198,7 +197,6 @@ __device__ __noinline__ void route_row_exact(const RouteParams& p, const float* 
     const double x = e < p.E ? (double)route_load(lg + e) : neg_inf<double>();
     const double a = exp(p.sigmoid ? -x : x - (double)m);
     const double sc = p.sigmoid ? 1.0 / (1.0 + a) : a / z;
-    score[i] = sc;
     const double w = sc + (double)(p.bias && e < p.E ? bias[e] : 0.f);
     const bool in = x > neg_inf<double>() && w > neg_inf<double>();
     v[i] = in ? double_order(w) : 0ull;
@@ -213,30 +211,20 @@ __device__ __noinline__ void route_row_exact(const RouteParams& p, const float* 
 #pragma unroll 1
     for (int g = 0; g < p.groups; ++g) {
       unsigned long long a = 0, b = 0;  // the lane's greatest two of the group
-      int ia = 0, ib = 0;
 #pragma unroll 1
       for (int i = 0; i < n; ++i) {
         const int e = i * 32 + lane;
         const unsigned long long k = e >= g * per && e < (g + 1) * per ? v[i] : 0ull;
-        const bool most = k > a, next = k > b;
-        b = most ? a : (next ? k : b);
-        ib = most ? ia : (next ? i : ib);
-        a = most ? k : a;
-        ia = most ? i : ia;
+        b = k > a ? a : (k > b ? k : b);
+        a = k > a ? k : a;
       }
       unsigned long long first = a;
       const unsigned owner = warp_best(first, lane);
       double s = first != 0 ? order_double(first) : neg_inf<double>();
       if (p.group_top == 2) {
         unsigned long long second = lane == owner ? b : a;
-        const int is = lane == owner ? ib : ia;
-        const unsigned other = warp_best(second, lane);
-        if (second != 0) {
-          // scores and biases apart: the same ones, paired the other way round, give the same sum
-          const int i0 = __shfl_sync(0xffffffffu, ia, (int)owner), i1 = __shfl_sync(0xffffffffu, is, (int)other);
-          s = __shfl_sync(0xffffffffu, score[i0], (int)owner) + __shfl_sync(0xffffffffu, score[i1], (int)other);
-          if (p.bias) s += (double)bias[i0 * 32 + (int)owner] + (double)bias[i1 * 32 + (int)other];
-        }
+        warp_best(second, lane);
+        if (second != 0) s += order_double(second);
       }
       if (lane == g) strength = s;
     }

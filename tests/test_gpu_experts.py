@@ -1104,24 +1104,3 @@ def test_sandwich_norm_skips_bad_rows_of_many(cuda_pkg, rows, D):
     want = k.sandwich_norm(x, y2, pg, pb, post_gamma=pg, routing=r)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     assert L.device_status(stream) == [0, 0, 0, 0]
-
-
-@pytest.mark.parametrize("scoring", ["sigmoid", "softmax"])
-def test_route_equal_strengths_take_the_lowest_group(cuda_pkg, scoring):
-    """Groups whose two best have the same logits and the same biases, paired the other
-    way round: equal sums, however they are rounded."""
-    g = _gen(41)
-    rows, G, per = 4000, 8, 4
-    pair = _randn(g, rows, 2, std=0.5)
-    logits = torch.full((rows, G, per), -6.0, device=DEV)
-    bias = torch.zeros(G, per, device=DEV)
-    for group in range(G):
-        logits[:, group, :2] = pair
-        bias[group, group % 2] = 0.003
-    logits[:, 0] -= 1.0  # weaker than the others
-    got = cuda_pkg.kernels.route_experts(logits.view(rows, -1), 2, scoring=scoring, bias=bias.view(-1), num_groups=G,
-                                         top_groups=1, group_score_top=2).experts
-    assert (got // per == 1).all()
-    got = cuda_pkg.kernels.route_experts(logits.view(rows, -1), 6, scoring=scoring, bias=bias.view(-1), num_groups=G,
-                                         top_groups=3, group_score_top=2).experts
-    assert torch.equal((got // per).sort(1)[0].cpu(), torch.tensor([1, 1, 2, 2, 3, 3], dtype=got.dtype).expand(rows, -1))
