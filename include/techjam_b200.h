@@ -279,11 +279,11 @@ TJ_API int64_t tj_expert_plan_ints(int rows, int top_k, int num_experts);
  * group's strength is the sum of its group_score_top (1 or 2) greatest
  * values, and only experts of the top_groups strongest groups stay.  The
  * top_k greatest values are chosen, greatest first; equal values (and groups)
- * in index order.  Values and strengths are compared as in 64-bit arithmetic,
- * not by their fp32 roundings; finite values that are equal there follow their
- * logits first (scores that saturate).  A NaN bias closes its expert.  weights
- * = s of the chosen (without bias), divided by their sum if renormalize, times
- * weight_scale.
+ * in index order.  Values and strengths are computed and compared in 64-bit
+ * arithmetic wherever their fp32 roundings could matter; finite values, and
+ * strengths of one value, that are equal there follow their logits first (scores
+ * that saturate).  A NaN bias closes its expert.  weights = s of the chosen
+ * (without bias), divided by their sum if renormalize, times weight_scale.
  * A logit of -inf closes an expert to the row: it has no part in the softmax
  * and is never chosen.  A row with fewer than top_k open experts has experts
  * -1 and weights 0 in its last places.  A row with a NaN logit (or +inf under

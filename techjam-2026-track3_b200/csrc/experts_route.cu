@@ -207,7 +207,9 @@ __device__ __noinline__ void route_row_exact(const RouteParams& p, const float* 
   blunt = __any_sync(0xffffffffu, blunt);
   if (p.groups > 1) {
     const int per = p.E / p.groups;
+    const bool by_logit = blunt && p.group_top == 1;
     double strength = neg_inf<double>();  // of group `lane`
+    float lead = 0.f;                     // strengths of one value: its greatest logit
 #pragma unroll 1
     for (int g = 0; g < p.groups; ++g) {
       unsigned long long a = 0, b = 0;  // the lane's greatest two of the group
@@ -226,13 +228,28 @@ __device__ __noinline__ void route_row_exact(const RouteParams& p, const float* 
         warp_best(second, lane);
         if (second != 0) s += order_double(second);
       }
+      if (by_logit && first != 0 && !isinf(s)) {
+        float l = neg_inf<float>();
+#pragma unroll 1
+        for (int i = 0; i < n; ++i) {
+          const int e = i * 32 + lane;
+          if (e >= g * per && e < (g + 1) * per && v[i] == first) l = fmaxf(l, route_load(lg + e));
+        }
+        l = row_max(l, 32);
+        if (lane == g) lead = l;
+      }
       if (lane == g) strength = s;
     }
     int above = 0;
 #pragma unroll 1
     for (int g = 0; g < p.groups; ++g) {
       const double o = __shfl_sync(0xffffffffu, strength, g);
-      above += o > strength || (o == strength && g < lane);
+      bool before = g < lane;
+      if (by_logit) {
+        const float l = __shfl_sync(0xffffffffu, lead, g);
+        before = l > lead || (l == lead && before);
+      }
+      above += o > strength || (o == strength && before);
     }
     const unsigned kept = __ballot_sync(0xffffffffu, lane < p.groups && above < p.top_groups);
 #pragma unroll 1

@@ -1104,3 +1104,20 @@ def test_sandwich_norm_skips_bad_rows_of_many(cuda_pkg, rows, D):
     want = k.sandwich_norm(x, y2, pg, pb, post_gamma=pg, routing=r)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     assert L.device_status(stream) == [0, 0, 0, 0]
+
+
+def test_route_groups_of_saturated_scores(cuda_pkg):
+    """Strengths of one value that are equal in 64 bits follow its logit, with any
+    bias as without one; equal logits go by group."""
+    g = _gen(42)
+    rows, G, per = 3000, 8, 6
+    logits = torch.randint(40, 60, (rows, G * per), generator=g, device=DEV).float()
+    kw = dict(scoring="sigmoid", num_groups=G, top_groups=3, group_score_top=1)
+    want = cuda_pkg.kernels.route_experts(logits, 8, **kw).experts
+    for odd in (0.0, -0.5):  # of one expert, which is then out of it
+        bias = torch.zeros(G * per, device=DEV)
+        bias[7] = odd
+        if odd:
+            logits[:, 7] = -50.0
+            want = cuda_pkg.kernels.route_experts(logits, 8, **kw).experts
+        assert torch.equal(cuda_pkg.kernels.route_experts(logits, 8, bias=bias, **kw).experts, want)
