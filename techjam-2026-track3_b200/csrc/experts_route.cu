@@ -620,7 +620,9 @@ __device__ void route_weights(const RouteParams& p, const int* flags, const floa
 #pragma unroll
     for (int i = 0; i < KL; ++i) {
       cm = fmaxf(cm, c[i]);
-      c[i] = e[i] >= 0 ? __fdividef(1.f, 1.f + expf(-c[i])) : 0.f;
+      // of exp(-|x|), which does not overflow: a far score beside small ones has a share
+      const float t = expf(-fabsf(c[i]));
+      c[i] = e[i] >= 0 ? __fdividef(c[i] < 0.f ? t : 1.f, 1.f + t) : 0.f;
       sum += c[i];
     }
     if (p.renorm) {

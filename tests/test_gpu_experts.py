@@ -1121,3 +1121,23 @@ def test_route_groups_of_saturated_scores(cuda_pkg):
             logits[:, 7] = -50.0
             want = cuda_pkg.kernels.route_experts(logits, 8, **kw).experts
         assert torch.equal(cuda_pkg.kernels.route_experts(logits, 8, bias=bias, **kw).experts, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [5, 3000])
+def test_route_far_sigmoids_keep_their_share(cuda_pkg, dtype, rows):
+    """Scores down to the subnormals beside small ones, renormalised: as _check_route, and
+    where a score is subnormal (steps of 2^-149, two of them in it) that over the sum."""
+    g = _gen(rows)
+    logits = (torch.randint(-200, -20, (rows, 12), generator=g, device=DEV) * 0.5).to(dtype)
+    logits[:, 3] = (torch.randint(-136, -120, (rows,), generator=g, device=DEV) * 0.5).to(dtype)
+    for k in (2, 5, 12):
+        for renorm in (True, False):
+            r = cuda_pkg.kernels.route_experts(logits, k, scoring="sigmoid", renormalize=renorm)
+            idx, w = _ref_route(logits, k, "sigmoid", renorm=renorm)
+            assert np.array_equal(r.experts.cpu().numpy(), idx)
+            total = 1.0 / (1.0 + np.exp(-np.take_along_axis(logits.double().cpu().numpy(), idx, 1)))
+            # sums below 1e-30 are of exponentials beside the greatest
+            step = np.where(total.sum(1) >= 1e-30, 2.0**-147 / total.sum(1), 2.0**-147)[:, None] if renorm else 2.0**-147
+            err = np.abs(r.weights.double().cpu().numpy() - w)
+            assert (err <= 32 * U32 * w + step).all(), (err / w).max()
