@@ -30,7 +30,10 @@
 // What bounds it: many rows per expert, the tensor cores under the power cap
 // (48000 x 1024 x 4096: 311 us, 1.29 PFLOP/s, where cuBLAS takes 291 us for the
 // product with one weight; GELU adds 36 us to FFN-in); few rows, the weights'
-// bytes (33 tokens x 4 of 64 experts: 223 MB in 41 us, 5.5 TB/s).
+// bytes (33 tokens x 4 of 64 experts, 55 reached: 231 MB in 41 us in FFN-in and 38 in
+// FFN-out back to back, 5.6 and 6.0 TB/s).
+// The hidden layer is rounded to 16 bits, since it is an operand of the second
+// product; outputs of gemm_experts are, since they are half the bytes.
 // The FFN-out of tj_expert_ffn leaves fp32 (expert_combine sums it).  With few
 // tiles its K is cut into `splits` parts, each its own tile with its own plane
 // of the output, which the combine adds up: no CTA waits for another, and one
@@ -779,7 +782,8 @@ static bool experts_gemm_pairs(int64_t slots, int num_experts) { return slots > 
 // can be reached), four K steps of 64 to a part at least.  One token, two experts,
 // K 4096: 8 parts, 19.8 us for the whole FFN instead of 25.5 with 16; above a
 // wave splitting only adds planes (33 tokens, 64 experts: 84.5 us unsplit, 87
-// and 90 us in two and four parts).
+// and 90 us in two and four parts).  148: a B200's SMs, not asked of the device,
+// since the workspace's size follows from the split.
 int experts_gemm_splits(int64_t slots, int num_experts, int n, int k) {
   if (experts_gemm_pairs(slots, num_experts)) return 1;
   const int64_t tiles = (slots < num_experts ? slots : num_experts) * ((n + kBM - 1) / kBM);

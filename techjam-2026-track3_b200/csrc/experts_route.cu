@@ -19,18 +19,19 @@
 // Plan: a stable counting sort of the (row, j) pairs by expert, in (row, j)
 // order inside an expert.  Each CTA of the router owns a chunk of rows and
 // writes its histogram; a second kernel (one CTA per chunk) adds up the
-// histograms of the chunks before it and ranks its own pairs with warp matches.  No atomic decides an order, so the plan is the same on every run.
-// Up to kRouteRowsPerCta rows fit one CTA, which then does both.
+// histograms of the chunks before it and ranks its own pairs with warp matches.
+// No atomic decides an order, so the plan is the same on every run.  Up to
+// kRouteRowsPerCta rows fit one CTA, which then does both.
 // The router reads rows * E logits and writes 16 bytes per pair.
 //
 // A CTA copies a tile of rows into shared memory (coalesced, transposed) and
 // gives each row L lanes, as many as it has threads for: one when the rows are
 // many, so that no instruction is spent on lanes agreeing, 32 for a few. Each
 // lane keeps the sorted best of its experts (i L + its number), then the lanes'
-// lists are merged.  90077 rows of 64 experts in groups, router and plan: 47 us;
-// a warp per row took 243 us, 8 lanes a row with eight experts each in registers
-// 80 us.  Bound by instructions and their latency (16.3 M for 60000 rows), not by
-// the 33 MB it moves (5 us).
+// lists are merged.  90077 rows of 64 experts in groups, router and plan: 47 us
+// back to back, 53 among others; a warp per row took 243 us, 8 lanes a row with
+// eight experts each in registers 80 us.  Bound by instructions and their latency
+// (16.1 M for 60000 rows), not by the 33 MB it moves (5 us).
 #include "common.cuh"
 #include "internal.h"
 
@@ -45,7 +46,9 @@ constexpr int kSortThreads = 1024;
 constexpr int kMaybe = 16;       // candidates a lane notes before it sorts them in
 constexpr int kPlanTile = 4096;  // pairs sorted at a time
 constexpr int kRouteRowsPerCta = 64;
-constexpr int kRouteMaxChunks = 148;  // one CTA per SM; also the rows of the histogram table
+// One CTA per SM of a B200, and the rows of the histogram table: the size of a plan
+// is asked for without a device.
+constexpr int kRouteMaxChunks = 148;
 constexpr uint16_t kNoChoice = 0xffff;
 constexpr int kRouteMaxExperts = 512;
 constexpr int kRouteMaxTopK = 32;

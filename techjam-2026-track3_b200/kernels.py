@@ -503,8 +503,8 @@ def route_experts(logits, top_k, *, scoring="softmax", bias=None, num_groups=1, 
     top_k experts and sorts the choices by expert.
 
     Scores are the row's softmax or sigmoid; the experts with the greatest
-    score + bias (bias: [E] float32) are chosen, equal values in index order,
-    and with num_groups > 1 only among the top_groups groups with the greatest
+    score + bias (bias: [E] float32) are chosen, as by 64-bit values, equal ones
+    by their logits and then in index order, and with num_groups > 1 only among the top_groups groups with the greatest
     sum of their group_score_top (1 or 2) best values.  Weights are the scores
     of the chosen, divided by their sum if renormalize, times weight_scale.  A
     logit of -inf closes an expert to the row (a row without enough open
